@@ -283,6 +283,68 @@ int tjx_ragged_paged_attention_bf16(const void* q, const void* keys, const void*
                                     int page_size, int pages_per_seq, int num_pages, float sm_scale, void* workspace,
                                     size_t workspace_bytes, tjx_stream_t stream);
 
+/* The next four entry points are a step over drafted tokens on the ragged paged cache (a tree of them for each
+ * sequence; one token, or a chunk of a prompt, is a path). They have no counterpart in the reference, whose step
+ * (examples/ragged_paged_attention.py:279-290) takes its tables, and its queries, keys and values, as they are to be. */
+
+/* Block tables and slot map of a step, from the requests' lengths. Sequence s has ctx_lens[s] positions in the cache on
+ * pages_held[s] pages (NULL: just enough) and brings q_lens[s] new tokens (negative lengths count as 0; tokens past row
+ * T are cut). One launch; functional except for page_indices.
+ *   kv_lens[s]   = ctx_lens[s] + q_lens[s]; cu_q_lens[S + 1] = first token of each sequence, then their number
+ *   page_indices int32[S * pages_per_seq], IN PLACE: the pages sequence s lacks, entries pages_held[s] and on, are taken
+ *                from the top of the stack free_pages[0 .. n_free[0]) in the order of the sequences; -1 where it is empty
+ *   pages_held_out[s] the pages it has then; n_free_out[2]: pages left on the stack, pages that were missing
+ *   positions[t] = ctx_lens[s] + the token's index in its sequence, or ctx_lens[s] + depths[t] where depths is given (a
+ *                drafted token's depth in its tree); slots[t] = its page * page_size + its row of the page, -1 where it
+ *                has no page (none left, or past the table). Rows behind the last token: position 0, slot -1.
+ * free_capacity is the length of free_pages. No output may overlap an input (NULL aside). At most 8192 sequences. */
+int tjx_rpa_plan(const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* pages_held, const int32_t* depths,
+                 int32_t* page_indices, const int32_t* free_pages, const int32_t* n_free, int free_capacity, int S, int T,
+                 int pages_per_seq, int page_size, int32_t* kv_lens, int32_t* cu_q_lens, int32_t* positions,
+                 int32_t* slots, int32_t* pages_held_out, int32_t* n_free_out, tjx_stream_t stream);
+
+/* RMS norm of every query and key head, its rotation by the token's position, and the cache write, in one pass:
+ * y = x * rsqrt(mean(x^2) + eps) * gamma (gammas NULL: y = x), then each pair (a, b) of the first `rot` elements becomes
+ * (a cos - b sin, a sin + b cos) with row positions[t] of cos_sin f32[max_positions, rot] (rot / 2 cosines, then rot / 2
+ * sines; the position is clamped to the table); all in f32, rounded to bf16 once. Pair i is elements i and i + rot / 2,
+ * or 2 i and 2 i + 1 if interleaved; elements from rot on are only normed.
+ *   q [T, H, D], k, v [T, Hkv, D] bf16, the last dimension dense; strides (HOST) = {q, k, v, q_out, k_out} x {token,
+ *   head} in elements, multiples of 4; q_gamma, k_gamma [D] bf16; q_out may be q, k_out may be k
+ *   to a cache: k_out NULL; k and v go to row slots[t] of kv_cache [n_slots, Hkv, 2, D] (a slot out of range writes
+ *   nothing; slots are distinct). Without one: v, slots and kv_cache NULL, k goes to k_out.
+ * Constraints: D 64, 128 or 256; rot % 8 == 0. */
+int tjx_norm_rope_bf16(const void* q, const void* k, const void* v, const int64_t* strides, const void* q_gamma,
+                       const void* k_gamma, const int32_t* positions, const float* cos_sin, const int32_t* slots,
+                       void* q_out, void* k_out, void* kv_cache, int T, int H, int Hkv, int D, int rot, int max_positions,
+                       int interleaved, int n_slots, float eps, tjx_stream_t stream);
+
+/* Bytes of scratch tjx_rpa_tree_attention_bf16 needs for these sizes. */
+size_t tjx_rpa_tree_attention_workspace_bytes(int T, int S, int H, int Hkv);
+
+/* Attention of drafted trees over the cache: rpa_decode for sequences that bring several tokens. Sequence
+ * s < distribution[0] has q_len = cu_q_lens[s + 1] - cu_q_lens[s] new tokens ("nodes"), node j at cache position
+ * kv_lens[s] - q_len + j (already written). Each attends, scores times sm_scale, to every position before those and to
+ * the nodes j whose bit (bit j % 32 of word j / 32) is set in its row of tree_mask int32[T, words]; a node past the
+ * words is seen by none. A row that sees nothing is zero; what hidden positions hold, NaN included, does not reach the
+ * result. Every other row of out [T, H, D] is q's (out may be q), as after tjx_rpa_decode_bf16: tjx_rpa_prefill_bf16
+ * with out as its q then serves the sequences from distribution[0] on.
+ *   workspace: at least tjx_rpa_tree_attention_workspace_bytes(...) bytes, 256-byte aligned
+ * Constraints: D == 128; H a multiple of Hkv, H / Hkv <= 128; page_size a multiple of 16; sm_scale > 0. */
+int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void* kv_cache, const int32_t* kv_lens,
+                                const int32_t* page_indices, const int32_t* cu_q_lens, const int32_t* tree_mask,
+                                const int32_t* distribution, int T, int S, int H, int Hkv, int D, int words,
+                                int page_size, int pages_per_seq, int num_pages, float sm_scale, void* workspace,
+                                size_t workspace_bytes, tjx_stream_t stream);
+
+/* The accepted path of each sequence's drafted tokens: with ctx = kv_lens[s] - q_len, cache row ctx + d becomes what row
+ * ctx + paths[s, d] holds, for d < n_accepted[s], IN PLACE, and out_lens[s] = ctx + n_accepted[s]. paths int32[S, P]
+ * ascends; a path ends in front of an entry that does not, or that is not one of the q_len nodes. n_accepted[s] < 0: the
+ * sequence keeps all its tokens, out_lens[s] = kv_lens[s]. Rows of kv_cache [num_pages, page_size, Hkv, 2, D] through
+ * page_indices [S * pages_per_seq]; a row without a page is not moved. out_lens must not overlap an input. */
+int tjx_rpa_commit_bf16(void* kv_cache, const int32_t* kv_lens, const int32_t* page_indices, const int32_t* cu_q_lens,
+                        const int32_t* paths, const int32_t* n_accepted, int32_t* out_lens, int S, int P, int Hkv, int D,
+                        int page_size, int pages_per_seq, int num_pages, tjx_stream_t stream);
+
 /* Which kernel tjx_mla_decode_bf16 launches from now on: 1 (the default) the tcgen05 kernel, 64 rows per CTA with
  * scores and output in TMEM; 0 the warp-level MMA kernel, 16 rows per CTA. An A/B switch for measurements: the two
  * agree to rounding. No counterpart in the reference. */

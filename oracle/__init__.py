@@ -26,6 +26,7 @@ from .decode import (
     paged_gqa_decode_ref,
     to_pages,
 )
+from .drafted import norm_rope_f64, pack_tree_mask, rpa_commit_ref, rpa_plan_ref, tree_attention_f64
 from .matmul import causal_matmul_ref, collective_row_order, matmul_ref
 from .rmsnorm import rmsnorm_matmul_f64, rmsnorm_matmul_ref
 from .rpa import (rpa_decode_f64, rpa_decode_ref, rpa_inputs, rpa_prefill_f64, rpa_prefill_ref, rpa_prefill_tiles,
@@ -52,18 +53,23 @@ __all__ = [
     "matmul_ref",
     "mla_decode_f64",
     "mla_decode_ref",
+    "norm_rope_f64",
+    "pack_tree_mask",
     "paged_gqa_decode_f64",
     "paged_gqa_decode_ref",
     "rmsnorm_matmul_f64",
     "rmsnorm_matmul_ref",
+    "rpa_commit_ref",
     "rpa_decode_f64",
     "rpa_decode_ref",
     "rpa_inputs",
+    "rpa_plan_ref",
     "rpa_prefill_f64",
     "rpa_prefill_ref",
     "rpa_prefill_tiles",
     "rpa_write_ref",
     "rpa_write_runs",
     "to_pages",
+    "tree_attention_f64",
     "walk_nest",
 ]

@@ -1,0 +1,147 @@
+"""A step over drafted tokens, on the CPU: the oracle on cases small enough to write down, and what the operators refuse
+before anything is launched."""
+
+import numpy as np
+import pytest
+import torch
+
+import oracle
+from tilejax_b200 import ops
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def test_the_plan_oracle_on_a_step_by_hand():
+    # Pages of 4. Sequence 0: 3 cached positions, 2 new ones: one more page. Sequence 1: new, 5 tokens: two pages, of
+    # which the stack holds none but one. Sequence 2: nothing new.
+    table = [7, -1, -1, -1, -1, -1, 2, -1, -1]
+    got = oracle.rpa_plan_ref([3, 0, 4], [2, 5, 0], table, [9, 5], [2], 4, 8)
+    assert [g.tolist() for g in got] == [[5, 5, 4], [0, 2, 7, 7], [3, 4, 0, 1, 2, 3, 4, 0],
+                                         [31, 20, 36, 37, 38, 39, -1, -1], [2, 1, 1], [0, 1],
+                                         [7, 5, -1, 9, -1, -1, 2, -1, -1]]
+
+
+def test_the_tree_oracle_is_causal_attention_on_a_path():
+    rng = np.random.default_rng(0)
+    q_lens, kv_lens = [5, 3], [12, 3]
+    inp = oracle.rpa_inputs(q_lens, kv_lens, heads=4, kv_heads=2, page_size=16, max_len=32, dtype=np.float64)
+    inp["distribution"][:] = [2, 2, 2]
+    mask = np.concatenate([oracle.pack_tree_mask(np.tril(np.ones((n, n), bool))) for n in q_lens])
+    names = ("kv_lens", "page_indices", "cu_q_lens")
+    got, size = oracle.tree_attention_f64(inp["q"], inp["kv_cache"], *(inp[n] for n in names), mask, [2, 2, 2], 0.1)
+    want = oracle.rpa_prefill_f64(inp["q"], inp["kv_cache"], *(inp[n] for n in names), np.array([0, 0, 2]), 0.1)
+    np.testing.assert_allclose(got, want, rtol=0, atol=1e-12)
+    assert (size >= np.abs(got) - 1e-12).all() and rng is not None
+
+
+def test_the_commit_oracle_moves_rows_along_the_path():
+    cache = np.arange(8, dtype=np.float64).reshape(2, 4, 1, 1, 1) * np.ones((1, 1, 1, 2, 1))
+    lens, after = oracle.rpa_commit_ref(cache, [7], [1, 0], [0, 5], np.array([[0, 2, 4, 3]]), [4])
+    # Positions 2.. of pages (1, 0): nodes are rows 6, 7, 0, 1, 2; kept are nodes 0, 2, 4 (3 does not ascend).
+    assert lens.tolist() == [5]
+    assert after[..., 0, 0, 0].reshape(-1).tolist() == [2, 1, 2, 3, 4, 5, 6, 0]
+
+
+def heads(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def refused(fn, good, bad):
+    with pytest.raises(ValueError, match="CUDA tensors"):  # everything else is in order
+        fn(**good())
+    for message, name, change in bad:
+        args = good()
+        args[name] = change(args[name])
+        with pytest.raises(ValueError, match=message):
+            fn(**args)
+
+
+def test_plan_refusals():
+    def good():
+        return dict(ctx_lens=i32(3, 0), q_lens=i32(2, 5), page_indices=i32(0, -1, -1, -1), free_pages=i32(1, 2, 3),
+                    n_free=i32(3), page_size=4, tokens=7, pages_held=i32(1, 0), depths=i32(*range(7)))
+
+    refused(ops.rpa_plan, good, [
+        ("ctx_lens must be an int32 vector", "ctx_lens", lambda t: t.long()),
+        ("q_lens must be an int32 vector", "q_lens", lambda t: t[None]),
+        (r"\(S,\)", "q_lens", lambda t: t[:1]),
+        ("pages_per_seq", "page_indices", lambda t: t[:3]),
+        ("number of free pages", "n_free", lambda t: t[:0]),
+        ("pages_held is", "pages_held", lambda t: t[:1]),
+        ("depths is", "depths", lambda t: t[:6]),
+        ("page_size must be positive", "page_size", lambda t: 0),
+        ("tokens not negative|depths is", "tokens", lambda t: -1),
+    ])
+
+
+def test_norm_rope_refusals():
+    def good():
+        return dict(q=heads(3, 4, 128), k=heads(3, 2, 128), q_gamma=heads(128), k_gamma=heads(128), positions=i32(0, 1, 2),
+                    cos_sin=torch.zeros(8, 128))
+
+    bad = [
+        (r"q is \(T, H, D\)", "q", lambda t: t[0]),
+        ("q must be bfloat16", "q", lambda t: t.float()),
+        ("k must be bfloat16", "k", lambda t: t[:2]),
+        ("strides multiples of 4", "q", lambda t: heads(3, 4, 130)[:, :, :128]),
+        ("last dimension must be dense", "q", lambda t: heads(3, 128, 4).transpose(1, 2)),
+        ("given together", "k_gamma", lambda t: None),
+        ("gammas are", "q_gamma", lambda t: t[:64]),
+        ("positions is", "positions", lambda t: t.long()),
+        ("cos_sin is", "cos_sin", lambda t: t.double()),
+        ("cos_sin is", "cos_sin", lambda t: t[:, :12]),
+        ("cos_sin is", "cos_sin", lambda t: torch.zeros(8, 136)),
+    ]
+    refused(ops.qk_norm_rope, good, bad)
+
+    def good_write():
+        return dict(**good(), v=heads(3, 2, 128), kv_cache=heads(4, 16, 2, 2, 128), slots=i32(3, 4, 5))
+
+    refused(ops.rpa_norm_rope_write, good_write, [b for b in bad if b[1] not in ("q", "k") or "strides" in b[0]] + [
+        ("k and v", "v", lambda t: t[:, :1]),
+        ("side by side", "kv_cache", lambda t: t.float()),
+        ("the cache's Hkv and D", "kv_cache", lambda t: heads(4, 16, 4, 2, 128)),
+        ("slots is", "slots", lambda t: t[:2]),
+    ])
+
+
+def test_tree_attention_refusals():
+    def good():
+        return dict(q=heads(3, 4, 128), kv_cache=heads(4, 16, 2, 2, 128), kv_lens=i32(9, 4), page_indices=i32(0, 1, 2, 3),
+                    cu_q_lens=i32(0, 2, 3), tree_mask=torch.zeros(3, 1, dtype=torch.int32), distribution=i32(2, 2, 2))
+
+    refused(ops.rpa_tree_attention, good, [
+        ("side by side", "kv_cache", lambda t: t[:, :, :, 0]),
+        ("page_indices is", "page_indices", lambda t: t[:3]),
+        ("must be int32", "kv_lens", lambda t: t.long()),
+        (r"q is \(T, H, D\)", "q", lambda t: t.float()),
+        (r"q is \(T, H, D\)", "q", lambda t: t[:, :, :64]),
+        ("cu_q_lens is", "cu_q_lens", lambda t: t[:2]),
+        ("cu_q_lens is", "distribution", lambda t: t.long()),
+        ("tree_mask is", "tree_mask", lambda t: t[:2]),
+        ("tree_mask is", "tree_mask", lambda t: t.bool()),
+    ])
+
+
+def test_commit_refusals():
+    def good():
+        return dict(kv_cache=heads(4, 16, 2, 2, 128), kv_lens=i32(9, 4), page_indices=i32(0, 1, 2, 3), cu_q_lens=i32(0, 2, 3),
+                    paths=torch.zeros(2, 2, dtype=torch.int32), n_accepted=i32(1, 1))
+
+    refused(ops.rpa_commit, good, [
+        ("side by side", "kv_cache", lambda t: t[:, :, :, 0]),
+        ("page_indices is", "page_indices", lambda t: t[:3]),
+        ("cu_q_lens is", "cu_q_lens", lambda t: t[:2]),
+        ("paths is", "paths", lambda t: t[:1]),
+        ("paths is", "paths", lambda t: t.long()),
+        ("n_accepted", "n_accepted", lambda t: t[:1]),
+    ])
+
+
+def test_overlap_is_seen_in_bytes():
+    base = torch.zeros(64, dtype=torch.int32)
+    assert ops._overlap(base[:10], base[9:]) and not ops._overlap(base[:10], base[10:])
+    assert ops._overlap(base.view(8, 8)[:, :2], base.view(8, 8)[:, 4:])  # ranges meet, though no element does
+    assert not ops._overlap(base[:0], base)

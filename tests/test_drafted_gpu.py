@@ -1,0 +1,401 @@
+"""A step over drafted tokens on the GPU: tables, norm and rotation with the cache write, tree attention, commit, each
+against plain NumPy in 64 bits, and a run of them together.
+
+Tolerances. Rounding to bf16 is off by at most 2^-8 of the value. Norm and rotation round once; before that f32 holds
+x, 1 / rms and the products to a few 2^-24 of what is added up (`size`): 2^-20 of it bounds them. Attention rounds the
+output once and each weight once, the latter relative to the weighted mean of |v| (`size`): 2^-8 of each; the weights'
+exponentials, the scores' f32 sums (128 products of |q k| up to about 60 before the scale, 1e-5 after it) and the joins
+of partial sums stay below 2^-11 of it together."""
+
+import numpy as np
+import pytest
+import torch
+from helpers import BF16, f64, rand_bf16, to_device, to_host
+
+import oracle
+from tilejax_b200 import ops
+from tilejax_b200._lib import NativeError
+
+pytestmark = pytest.mark.gpu
+
+
+def dev32(*values):
+    return torch.tensor(np.asarray(values[0] if len(values) == 1 else values), dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------ tables
+
+
+PLANS = [  # (ctx, new, page_size, pages_per_seq, tokens - sum(new), pages short, held or None, depths)
+    ([3], [1], 4, 2, 0, 0, None, False),
+    ([3, 0, 4, 8], [2, 5, 0, 1], 4, 3, 3, 0, None, True),
+    ([0, 0], [0, 0], 16, 1, 2, 0, None, False),                       # nothing to do, padding rows
+    ([5, 40, 17], [30, 9, 100], 16, 8, 0, 4, None, False),            # the stack runs out on the way
+    ([5, 40, 17], [30, 9, 100], 16, 8, 0, 99, None, False),           # an empty stack
+    ([30, 60], [10, 10], 16, 4, 0, 0, None, False),                   # the second sequence passes its table's end
+    ([16, 20], [3, 3], 16, 4, 1, 0, [3, 1], True),                    # pages held ahead, and fewer than used
+    ([2, 3, 4], [4, 4, 4], 16, 2, -5, 0, None, False),                # fewer rows than new tokens
+    (list(range(0, 1500, 7)), [1 + 13 * (i % 5) for i in range(215)], 16, 100, 7, 0, None, True),
+    (list(range(2500)), [i % 3 for i in range(2500)], 48, 60, 0, 1, None, False),  # more than a round of the scan
+]
+
+
+@pytest.mark.parametrize("case", PLANS)
+def test_plan_is_exact(case):
+    ctx, new, page, pps, extra, short, held, with_depths = case
+    rng = np.random.default_rng(len(ctx))
+    S, T = len(ctx), sum(new) + extra
+    have = [min(-(-c // page), pps) for c in ctx] if held is None else held
+    order = rng.permutation(sum(have) + sum(-(-n // page) + 1 for n in new) + 5)
+    table = np.full((S, pps), -1, np.int32)
+    at = 0
+    for s, n in enumerate(have):
+        table[s, :n] = order[at : at + n]
+        at += n
+    need = sum(max(min(-(-(c + n) // page), pps) - h, 0) for c, n, h in zip(ctx, new, have))
+    free = order[at:]
+    n_free = [max(need - short, 0)] if short else [len(free)]
+    depths = rng.integers(0, 6, T).astype(np.int32) if with_depths else None
+    want = oracle.rpa_plan_ref(ctx, new, table.reshape(-1), free, n_free, page, T, held, depths)
+    pages = dev32(table.reshape(-1))
+    args = (dev32(ctx), dev32(new), pages, dev32(free), dev32(n_free), page, T)
+    kw = dict(pages_held=None if held is None else dev32(held), depths=None if depths is None else dev32(depths))
+    got = ops.rpa_plan(*args, **kw)
+    for name, g, w in zip((*got._fields, "page_indices"), (*got, pages), want):
+        np.testing.assert_array_equal(to_host(g), w, err_msg=name)
+    # Again, into the same step: the table holds the pages already, the inputs say what was held.
+    again = ops.rpa_plan(*args, **kw, out=got)
+    for g, w in zip((*again, pages), want):
+        np.testing.assert_array_equal(to_host(g), w)
+
+
+def test_plan_refuses_an_output_among_its_inputs():
+    ctx = dev32([3, 4])
+    args = (ctx, dev32([1, 1]), dev32([0, -1, 1, -1]), dev32([2, 3]), dev32([2]), 4, 2)
+    step = ops.rpa_plan(*args)
+    with pytest.raises(ValueError, match="overlaps an input"):
+        ops.rpa_plan(*args, out=step._replace(kv_lens=ctx))
+    with pytest.raises(ValueError, match="other sizes"):
+        ops.rpa_plan(*args, out=step._replace(slots=step.slots[:1]))
+    S = 8193
+    with pytest.raises(NativeError, match="more than 8192 sequences"):
+        ops.rpa_plan(dev32([0] * S), dev32([1] * S), dev32([0] * S), dev32([0]), dev32([1]), 4, S)
+
+
+# ------------------------------------------------------------------------------------------ norm, rotation, write
+
+
+def angles(positions, rot):
+    a = np.arange(positions)[:, None] * 10000.0 ** (-np.arange(rot // 2) * 2 / max(rot, 1))
+    return np.concatenate([np.cos(a), np.sin(a)], 1).astype(np.float32)
+
+
+def close(got, want, size, slack=2.0**-20):
+    got = f64(got)
+    assert np.isfinite(got).all()
+    over = np.abs(got - want) - (2.0**-8 * np.abs(want) + slack * size)
+    assert over.max(initial=-1.0) <= 1e-30, over.max()
+
+
+@pytest.mark.parametrize(("T", "H", "Hkv", "D", "rot", "interleaved", "norm"), [
+    (1, 32, 8, 128, 128, False, True),
+    (7, 32, 8, 128, 128, True, True),
+    (5, 3, 1, 128, 64, False, True),       # half of the head, an odd number of rows
+    (3, 28, 4, 128, 96, True, False),
+    (33, 5, 5, 64, 64, False, True),
+    (9, 8, 2, 256, 128, False, True),
+    (2, 1, 1, 256, 8, True, True),
+    (700, 7, 3, 64, 32, True, False),
+    (4, 4, 4, 128, 0, False, True),        # the norm alone
+])
+def test_norm_and_rotation(T, H, Hkv, D, rot, interleaved, norm):
+    rng = np.random.default_rng(T)
+    qkv = rand_bf16((T, H + 2 * Hkv, D), T, 3.0)
+    gq, gk = (rand_bf16((D,), 5 + i) for i in range(2)) if norm else (None, None)
+    table = angles(100, rot)
+    positions = rng.integers(-5, 130, T).astype(np.int32)  # some past the table: clamped
+    q, k, v = qkv[:, :H], qkv[:, H : H + Hkv], qkv[:, H + Hkv :]
+    want_q, size_q = oracle.norm_rope_f64(q, gq, positions, table, 1e-5, interleaved)
+    want_k, size_k = oracle.norm_rope_f64(k, gk, positions, table, 1e-5, interleaved)
+    packed = to_device(qkv)
+    dq, dk, dv = packed[:, :H], packed[:, H : H + Hkv], packed[:, H + Hkv :]  # views: strides of the packed rows
+    gammas = [None if g is None else to_device(g) for g in (gq, gk)]
+    args = (*gammas, to_device(positions), to_device(table))
+    got = ops.qk_norm_rope(dq, dk, *args, eps=1e-5, interleaved=interleaved)
+    close(to_host(got[0]), want_q, size_q)
+    close(to_host(got[1]), want_k, size_k)
+    # To the cache, some tokens without a slot: the same keys, the values as they are, and nothing else.
+    page = 16
+    pages = -(-2 * T // page) + 1
+    cache = rand_bf16((pages, page, Hkv, 2, D), 9)
+    slots = rng.permutation(pages * page)[:T].astype(np.int32)
+    slots[::5] = -1
+    slots[3::7] = pages * page
+    dcache = to_device(cache)
+    got_q, same = ops.rpa_norm_rope_write(dq, dk, dv, *args, dcache, to_device(slots), eps=1e-5, interleaved=interleaved)
+    assert same is dcache and torch.equal(got_q, got[0])
+    rows = cache.reshape(-1, Hkv, 2, D)
+    for t in range(T):
+        if 0 <= slots[t] < pages * page:
+            rows[slots[t], :, 0], rows[slots[t], :, 1] = to_host(got[1][t]), v[t]
+    np.testing.assert_array_equal(to_host(dcache).view(np.uint16), cache.view(np.uint16))
+    np.testing.assert_array_equal(to_host(packed).view(np.uint16), qkv.view(np.uint16))  # the operands are left alone
+    # In place, inside the packed rows.
+    ops.qk_norm_rope(dq, dk, *args, eps=1e-5, interleaved=interleaved, out=(dq, dk))
+    assert torch.equal(dq, got[0]) and torch.equal(dk, got[1])
+    np.testing.assert_array_equal(to_host(dv).view(np.uint16), v.view(np.uint16))
+
+
+def test_norm_and_rotation_refuse_overlapping_outputs_and_unknown_heads():
+    q, k = (torch.zeros(4, h, 128, dtype=torch.bfloat16, device="cuda") for h in (8, 2))
+    args = (None, None, dev32([0] * 4), torch.zeros(4, 128, device="cuda"))
+    with pytest.raises(ValueError, match="memory of its own"):
+        ops.qk_norm_rope(q[:2], k[:2], None, None, dev32([0] * 2), args[3], out=(q[1:3], k[:2]))
+    with pytest.raises(ValueError, match="memory of its own"):
+        ops.qk_norm_rope(q, k, *args, out=(q, q[:, :2]))
+    with pytest.raises(NativeError, match="64, 128 or 256"):
+        ops.qk_norm_rope(q[:, :, :32].contiguous(), k[:, :, :32].contiguous(), None, None, args[2],
+                         torch.zeros(4, 32, device="cuda"))
+    with pytest.raises(NativeError, match="eps"):
+        ops.qk_norm_rope(q, k, *args, eps=float("nan"))
+
+
+# ------------------------------------------------------------------------------------------ tree attention
+
+
+def tree(n, rng, empty=False):
+    sees = np.zeros((n, n), bool)
+    for i in range(n):
+        if i:
+            sees[i] = sees[rng.integers(0, i)]
+        sees[i, i] = True
+    if empty:
+        sees[n // 2] = False
+    return sees
+
+
+def tree_case(q_lens, kv_lens, heads, kv_heads, page_size, *, words=None, max_seqs=None, extra=0, empty=False, seed=0,
+              poison=True, scale=1.0):
+    """Inputs of a step of trees; with `poison`, NaN and infinities wherever no row looks: rows behind a sequence's last
+    position, pages of nobody."""
+    rng = np.random.default_rng(seed)
+    S = len(q_lens) if max_seqs is None else max_seqs
+    T = sum(q_lens)
+    used = [-(-n // page_size) for n in kv_lens]
+    pps = max(1, *used) + 1
+    pool = sum(used) + 2
+    order = rng.permutation(pool)
+    table = rng.integers(-3, pool + 3, (S, pps)).astype(np.int32)  # entries past a sequence's pages: anything
+    cache = (rng.standard_normal((pool, page_size, kv_heads, 2, 128), np.float32)).astype(BF16)
+    at = 0
+    if poison:
+        cache[order[sum(used):]] = np.nan
+    for s, n in enumerate(used):
+        table[s, :n] = order[at : at + n]
+        at += n
+        if poison and n:
+            tail = kv_lens[s] - (n - 1) * page_size
+            cache[table[s, n - 1], tail:] = np.array([np.nan, np.inf, -np.inf])[rng.integers(0, 3, cache[0, tail:].shape)].astype(BF16)
+    cu = np.full(S + 1, T, np.int32)
+    cu[: len(q_lens) + 1] = np.concatenate([[0], np.cumsum(q_lens)])
+    lens = np.zeros(S, np.int32)
+    lens[: len(kv_lens)] = kv_lens
+    words = max(1, -(-max(q_lens) // 32)) if words is None else words
+    masks = [oracle.pack_tree_mask(tree(n, rng, empty), words) for n in q_lens] + [np.zeros((extra, words), np.int32)]
+    q = (scale * rng.standard_normal((T + extra, heads, 128), np.float32)).astype(BF16)
+    return dict(q=q, kv_cache=cache, kv_lens=lens, page_indices=table.reshape(-1), cu_q_lens=cu,
+                tree_mask=np.concatenate(masks), distribution=np.array([len(q_lens)] * 3, np.int32))
+
+
+def check_tree(inp, sm_scale=128**-0.5):
+    dev = {k: to_device(v) for k, v in inp.items()}
+    got = ops.rpa_tree_attention(**dev, sm_scale=sm_scale)
+    assert ops.device_status() == 0
+    want, size = oracle.tree_attention_f64(*inp.values(), sm_scale)
+    close(to_host(got), want, size, 2.0**-8 + 2.0**-11)
+    np.testing.assert_array_equal(to_host(dev["q"]).view(np.uint16), inp["q"].view(np.uint16))
+    rest = int(inp["cu_q_lens"][inp["distribution"][0]])
+    np.testing.assert_array_equal(to_host(got)[rest:].view(np.uint16), inp["q"][rest:].view(np.uint16))
+    in_place = dev["q"].clone()
+    same = ops.rpa_tree_attention(**{**dev, "q": in_place}, sm_scale=sm_scale, out=in_place)
+    assert same is in_place and torch.equal(in_place.view(torch.int16), got.view(torch.int16))
+    return got
+
+
+TREES = {
+    "one token": ([1], [1], 8, 2, 16),
+    "one token, long": ([1], [1000], 8, 2, 16),
+    "no prefix": ([9], [9], 4, 4, 32),
+    "a block exactly": ([16], [128], 16, 2, 64),
+    "a block and one": ([16], [129], 16, 2, 64),
+    "a page inside": ([5, 3, 8], [63, 64, 65], 8, 2, 48),
+    "ragged": ([8, 1, 17, 30], [700, 3, 17, 333], 32, 8, 16),
+    "seven to a head": ([25, 3, 19], [200, 61, 129], 28, 4, 48),
+    "three to a head": ([43, 44], [300, 90], 3, 1, 16),
+    "five to a head": ([26], [77], 20, 4, 16),
+    "one to a head": ([64, 2], [190, 66], 2, 2, 128),
+    "two row tiles": ([32], [500], 8, 1, 32),
+    "many rows": ([70, 33], [400, 100], 8, 1, 256),
+    "wide group": ([3, 9], [260, 40], 128, 1, 16),
+    "uneven group": ([2, 5], [70, 20], 100, 1, 16),
+    "split": ([12], [9000], 8, 2, 16),
+}
+
+
+@pytest.mark.parametrize("name", TREES)
+def test_tree_attention_matches_float64(name):
+    check_tree(tree_case(*TREES[name], seed=len(name)))
+
+
+@pytest.mark.parametrize(("kw", "case"), [
+    (dict(empty=True), ([6, 5], [6, 70], 8, 2, 16)),           # a row that sees nothing (no prefix), one that sees only it
+    (dict(max_seqs=7, extra=5), ([4, 9], [40, 9], 8, 2, 16)),  # a padded batch: empty sequences, rows behind the last
+    (dict(words=1), ([40], [300], 4, 2, 16)),                  # nodes past the mask's words: seen by none
+    (dict(words=5), ([3], [30], 4, 2, 16)),
+    (dict(scale=30.0), ([8, 16], [500, 90], 8, 2, 16)),        # scores far apart: the running maximum moves often
+])
+def test_tree_attention_at_its_edges(kw, case):
+    check_tree(tree_case(*case, **kw))
+
+
+def test_a_longer_tree_than_its_cache_and_lengths_past_the_table():
+    inp = tree_case([6, 4], [20, 30], 8, 2, 16)
+    inp["kv_lens"][0] = 4          # four positions for six nodes: the first two are in no cache row
+    check_tree(inp)
+    inp["kv_lens"][:] = [0, 30]    # an empty sequence that brings tokens: its rows are zero
+    assert not check_tree(inp)[:6].any()
+    # A length past the table: what the table holds is attended to.
+    inp = tree_case([2], [60], 4, 2, 16, poison=False)
+    inp["page_indices"][-1] = 0
+    inp["kv_lens"][0] = 100
+    check_tree(inp)
+
+
+def test_nan_in_a_hidden_node_stays_there():
+    # Node 2 of the tree holds NaN and infinity: rows that see it are NaN, those that do not are as without it.
+    for nodes, group, ctx in ((6, 4, 50), (40, 8, 200), (40, 8, 24)):
+        inp = tree_case([nodes], [ctx + nodes], group, 1, 16, seed=nodes)
+        sees = np.zeros((nodes, nodes), bool)
+        for i in range(nodes):
+            sees[i, i] = True
+            sees[i, i % 3] = True
+        inp["tree_mask"][:] = oracle.pack_tree_mask(sees, inp["tree_mask"].shape[1])
+        spot = ctx + 2
+        row = inp["kv_cache"][inp["page_indices"][spot // 16], spot % 16]
+        row[0, 1, :64], row[0, 1, 64:] = np.nan, np.inf
+        dev = {k: to_device(v) for k, v in inp.items()}
+        got = f64(to_host(ops.rpa_tree_attention(**dev, sm_scale=128**-0.5)))
+        with np.errstate(invalid="ignore"):
+            want, size = oracle.tree_attention_f64(*inp.values(), 128**-0.5)
+        blind = ~sees[:, 2]
+        close(got[blind], want[blind], size[blind], 2.0**-8 + 2.0**-11)
+        assert np.isnan(got[~blind][..., :64]).all() and np.isposinf(got[~blind][..., 64:]).all()
+
+
+def test_tree_attention_refuses_what_it_cannot_do():
+    dev = {k: to_device(v) for k, v in tree_case([4], [40], 8, 2, 16).items()}
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(NativeError, match="sm_scale"):
+            ops.rpa_tree_attention(**dev, sm_scale=scale)
+    with pytest.raises(NativeError, match="multiple of the KV heads"):
+        ops.rpa_tree_attention(**{**dev, "q": torch.zeros(4, 7, 128, dtype=torch.bfloat16, device="cuda")})
+    with pytest.raises(NativeError, match="multiple of 16"):
+        ops.rpa_tree_attention(**{**dev, "kv_cache": torch.zeros(4, 24, 2, 2, 128, dtype=torch.bfloat16, device="cuda")})
+    with pytest.raises(NativeError, match="at most 128"):
+        ops.rpa_tree_attention(**{**dev, "q": torch.zeros(4, 258, 128, dtype=torch.bfloat16, device="cuda")})
+    with pytest.raises(ValueError, match="memory of its own"):
+        wide = torch.zeros(6, 8, 128, dtype=torch.bfloat16, device="cuda")
+        ops.rpa_tree_attention(**{**dev, "q": wide[:4]}, out=wide[2:])
+
+
+# ------------------------------------------------------------------------------------------ commit
+
+
+def test_commit_is_exact():
+    rng = np.random.default_rng(4)
+    kv_heads, page = 3, 16
+    for seed, (q_lens, kv_lens) in enumerate([([5], [5]), ([1, 16, 64, 9, 4, 40], [30, 100, 64, 10, 4, 300])]):
+        inp = tree_case(q_lens, kv_lens, 3, kv_heads, page, seed=seed, poison=False)
+        P = 24
+        paths = np.stack([np.sort(rng.permutation(80)[:P]) for _ in q_lens]).astype(np.int32)
+        for s, n in enumerate(q_lens):
+            take = min(n, P)
+            paths[s, :take] = np.sort(rng.permutation(n)[:take])
+        accepted = np.array([min(n, P) for n in q_lens], np.int32)
+        if len(q_lens) > 1:
+            accepted[3], accepted[4] = -1, 0
+            accepted[5] = 99            # more than the path holds
+            paths[1, 4] = paths[1, 3]   # does not ascend: the path ends there
+        names = ("kv_cache", "kv_lens", "page_indices", "cu_q_lens")
+        want_lens, want = oracle.rpa_commit_ref(*(inp[n] for n in names), paths, accepted)
+        dev = [to_device(inp[n]) for n in names]
+        out = torch.empty(len(q_lens), dtype=torch.int32, device="cuda")
+        lens = ops.rpa_commit(*dev, to_device(paths), to_device(accepted), out=out)
+        assert lens is out
+        np.testing.assert_array_equal(to_host(lens), want_lens)
+        np.testing.assert_array_equal(to_host(dev[0]).view(np.uint16), want.view(np.uint16))
+        with pytest.raises(ValueError, match="overlaps an input"):
+            ops.rpa_commit(*dev, to_device(paths), to_device(accepted), out=dev[1])
+
+
+# ------------------------------------------------------------------------------------------ together
+
+
+def test_two_steps_of_drafted_tokens_with_a_prompt_beside_them():
+    # Plan, norm + rotation + write, tree attention, prefill of the one prompt, commit; then a step on what was kept. The
+    # cache the second step sees is checked against the tokens that were kept, its attention against float64.
+    rng = np.random.default_rng(11)
+    H, Hkv, page, pps, scale = 8, 2, 128, 4, 128**-0.5
+    table = angles(600, 128)
+    ctx, nodes, prompt = [100, 250], [7, 12], 60
+    total = 16
+    pages = dev32(np.full(3 * pps, -1))
+    cache = torch.zeros(total, page, Hkv, 2, 128, dtype=torch.bfloat16, device="cuda")
+    free, n_free = dev32(rng.permutation(total)), dev32([total])
+    gq, gk = (to_device(rand_bf16((128,), i)) for i in (1, 2))
+    cos_sin = to_device(table)
+
+    def step(ctx_lens, new, depths, n_free, held, seed):
+        T = sum(new)
+        qkv = to_device(rand_bf16((T, H + 2 * Hkv, 128), seed))
+        plan = ops.rpa_plan(ctx_lens, dev32(new), pages, free, n_free, page, T, pages_held=held,
+                            depths=None if depths is None else dev32(depths))
+        q, _ = ops.rpa_norm_rope_write(qkv[:, :H], qkv[:, H : H + Hkv], qkv[:, H + Hkv :], gq, gk, plan.positions,
+                                       cos_sin, cache, plan.slots)
+        return plan, q
+
+    # The prefixes themselves, by the same operators: chunks of a prompt are paths.
+    plan, _ = step(dev32([0, 0, 0]), [*ctx, 0], None, n_free, dev32([0, 0, 0]), 1)
+    sees = [tree(n, rng) for n in nodes]
+    depths = np.concatenate([s.sum(1) - 1 for s in sees] + [np.arange(prompt)])
+    first, q = step(plan.kv_lens, [*nodes, prompt], depths, plan.n_free, plan.pages_held, 2)
+    np.testing.assert_array_equal(to_host(first.positions)[: nodes[0]], ctx[0] + sees[0].sum(1) - 1)
+    mask = to_device(np.concatenate([oracle.pack_tree_mask(s) for s in sees] + [np.zeros((prompt, 1), np.int32)]))
+    dist = dev32([2, 2, 3])
+    out = ops.rpa_tree_attention(q, cache, first.kv_lens, pages, first.cu_q_lens, mask, dist, scale)
+    out = ops.rpa_prefill(out, cache, first.kv_lens, pages, first.cu_q_lens, dist, scale, out=out)
+    assert ops.device_status() == 0
+    host = [to_host(x) for x in (q, cache, first.kv_lens, pages, first.cu_q_lens)]
+    want, size = oracle.tree_attention_f64(*host, to_host(mask), [2, 2, 3], scale)
+    trees = sum(nodes)
+    close(to_host(out)[:trees], want[:trees], size[:trees], 2.0**-8 + 2.0**-11)
+    want = oracle.rpa_prefill_f64(*host, np.array([2, 2, 3]), scale)
+    assert np.abs(f64(to_host(out))[trees:] - want[trees:]).max() <= 2e-2
+
+    # Keep the longest path of each tree; the prompt keeps all its tokens.
+    paths, accepted = np.zeros((3, 12), np.int32), np.array([0, 0, -1], np.int32)
+    for s in range(2):
+        deepest = np.flatnonzero(sees[s][int(sees[s].sum(1).argmax())])
+        paths[s, : len(deepest)], accepted[s] = deepest, len(deepest)
+    before = to_host(cache)
+    lens = ops.rpa_commit(cache, first.kv_lens, pages, first.cu_q_lens, to_device(paths), to_device(accepted))
+    want_lens, want_cache = oracle.rpa_commit_ref(before, *host[2:], paths, accepted)
+    np.testing.assert_array_equal(to_host(lens), want_lens)
+    np.testing.assert_array_equal(to_host(cache).view(np.uint16), want_cache.view(np.uint16))
+    second, q = step(lens, [3, 3, 1], [0, 1, 1, 0, 1, 2, 0], first.n_free, first.pages_held, 3)
+    mask = to_device(np.concatenate([oracle.pack_tree_mask(tree(n, rng)) for n in (3, 3, 1)]))
+    out = ops.rpa_tree_attention(q, cache, second.kv_lens, pages, second.cu_q_lens, mask, dev32([3, 3, 3]), scale)
+    host = [to_host(x) for x in (q, cache, second.kv_lens, pages, second.cu_q_lens, mask)]
+    want, size = oracle.tree_attention_f64(*host, [3, 3, 3], scale)
+    close(to_host(out), want, size, 2.0**-8 + 2.0**-11)
+    assert to_host(second.n_free)[1] == 0

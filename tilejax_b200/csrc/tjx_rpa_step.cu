@@ -1,0 +1,441 @@
+// What a step on the ragged paged cache (examples/ragged_paged_attention.py: pages of page_size positions, each
+// position's heads with key and value side by side) needs around its attention, made on the device from the requests'
+// lengths and the projection's output:
+//   rpa_plan_kernel        block tables, slot map, positions and token offsets of the step from the requests' lengths
+//   norm_rope_kernel       RMS norm of every query and key head and its rotation by the token's position; keys and
+//                          values straight into their cache rows
+//   rpa_commit_kernel      the rows of an accepted path of drafted tokens moved behind the cached prefix
+#include <algorithm>
+
+#include "tjx_host.cuh"
+#include "tjx_ptx.cuh"
+
+#include "../../include/tilejax_b200.h"
+
+namespace tjx {
+
+// ------------------------------------------------------------------------------------------ block tables and slots
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_MAX_SEQS = 8192;  // two int32 prefix arrays in shared memory
+
+struct PlanParams {
+  const int32_t *ctx_lens, *q_lens, *held, *depths;  // held, depths: or null
+  int32_t* page_indices;
+  const int32_t *free_pages, *n_free;
+  int free_capacity;
+  int S, T, pages_per_seq, page_size;
+  int32_t *kv_lens, *cu_q_lens, *positions, *slots, *held_out, *n_free_out;
+};
+
+// Last entry of the nondecreasing prefix array a[0..n) that is <= x (a[0] <= x).
+__device__ __forceinline__ int prefix_find(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Every CTA scans all sequences (new tokens, and pages a sequence lacks) into shared memory and then takes its share
+// of the tokens and of the pages handed out; CTA 0 also writes what there is one of per sequence. Nothing a CTA reads
+// is written by another: table entries below a sequence's held pages are only read, those handed out only written
+// (a token on such a page takes it from the free list itself). Bound by latency: a load, a scan, a search and two
+// dependent loads.
+__global__ void __launch_bounds__(PLAN_THREADS) rpa_plan_kernel(const PlanParams p) {
+  extern __shared__ int plan_smem[];
+  int* cu = plan_smem;            // [S + 1] first token of each sequence, clipped to T
+  int* lack = plan_smem + p.S + 1;  // [S + 1] first fresh page of each sequence
+  __shared__ long long warp_q[32];
+  __shared__ int warp_n[32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  long long carry_q = 0;
+  int carry_n = 0;
+  const int free_now = min(max(p.n_free[0], 0), p.free_capacity);
+  for (int s0 = 0; s0 < p.S; s0 += PLAN_THREADS) {
+    const int s = s0 + t;
+    int q = 0, need = 0, ctx = 0, held = 0;
+    if (s < p.S) {
+      ctx = max(p.ctx_lens[s], 0), q = max(p.q_lens[s], 0);
+      const int cached = static_cast<int>((static_cast<long long>(ctx) + p.page_size - 1) / p.page_size);
+      held = min(max(p.held != nullptr ? p.held[s] : cached, 0), p.pages_per_seq);
+    }
+    // The scan of the new tokens comes first: a sequence past row T adds what fits.
+    long long iq = q;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xFFFFFFFFu, iq, d);
+      if (lane >= d) iq += y;
+    }
+    if (lane == 31) warp_q[warp] = iq;
+    __syncthreads();
+    if (warp == 0) {
+      long long w = warp_q[lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xFFFFFFFFu, w, d);
+        if (lane >= d) w += y;
+      }
+      warp_q[lane] = w;
+    }
+    __syncthreads();
+    const long long end_q = carry_q + (warp > 0 ? warp_q[warp - 1] : 0) + iq;
+    const int first = static_cast<int>(min(end_q - q, static_cast<long long>(p.T)));
+    const int last = static_cast<int>(min(end_q, static_cast<long long>(p.T)));
+    const int len = static_cast<int>(min(static_cast<long long>(ctx) + (last - first), 0x7FFFFFFFll));
+    if (s < p.S) {
+      const long long pages = (static_cast<long long>(len) + p.page_size - 1) / p.page_size;
+      need = max(static_cast<int>(min(pages, static_cast<long long>(p.pages_per_seq))) - held, 0);
+    }
+    int in = need;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, in, d);
+      if (lane >= d) in += y;
+    }
+    if (lane == 31) warp_n[warp] = in;
+    __syncthreads();
+    if (warp == 0) {
+      int w = warp_n[lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xFFFFFFFFu, w, d);
+        if (lane >= d) w += y;
+      }
+      warp_n[lane] = w;
+    }
+    __syncthreads();
+    const int before = carry_n + (warp > 0 ? warp_n[warp - 1] : 0) + in - need;
+    if (s < p.S) {
+      cu[s] = first;
+      lack[s] = before;
+      if (blockIdx.x == 0) {
+        p.kv_lens[s] = len;
+        p.cu_q_lens[s] = first;
+        p.held_out[s] = held + min(max(free_now - before, 0), need);
+      }
+    }
+    carry_q += warp_q[31];
+    carry_n += warp_n[31];
+    __syncthreads();  // the warps' sums are overwritten by the next round
+  }
+  const int total = static_cast<int>(min(carry_q, static_cast<long long>(p.T)));
+  if (t == 0) {
+    cu[p.S] = total, lack[p.S] = carry_n;
+    if (blockIdx.x == 0) {
+      p.cu_q_lens[p.S] = total;
+      p.n_free_out[0] = max(free_now - carry_n, 0);
+      p.n_free_out[1] = max(carry_n - free_now, 0);
+    }
+  }
+  __syncthreads();
+  const int step = static_cast<int>(gridDim.x) * PLAN_THREADS, me = static_cast<int>(blockIdx.x) * PLAN_THREADS + t;
+  auto held_of = [&](int s) {
+    const int cached = static_cast<int>((static_cast<long long>(max(p.ctx_lens[s], 0)) + p.page_size - 1) / p.page_size);
+    return min(max(p.held != nullptr ? p.held[s] : cached, 0), p.pages_per_seq);
+  };
+  // The k-th page handed out comes off the top of the free stack, or is missing.
+  auto fresh = [&](int k) { return k < free_now ? p.free_pages[free_now - 1 - k] : -1; };
+  for (int k = me; k < carry_n; k += step) {
+    const int s = prefix_find(lack, p.S + 1, k);
+    p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + held_of(s) + (k - lack[s])] = fresh(k);
+  }
+  for (int i = me; i < p.T; i += step) {
+    int position = 0, slot = -1;
+    if (i < total) {
+      const int s = prefix_find(cu, p.S + 1, i);
+      const int ctx = max(p.ctx_lens[s], 0), index = i - cu[s];
+      const unsigned place = static_cast<unsigned>(ctx) + static_cast<unsigned>(index);
+      const unsigned page = place / static_cast<unsigned>(p.page_size), row = place % static_cast<unsigned>(p.page_size);
+      position = p.depths != nullptr ? ctx + p.depths[i] : static_cast<int>(place);
+      if (page < static_cast<unsigned>(p.pages_per_seq)) {
+        const int held = held_of(s);
+        const int entry = static_cast<int>(page) < held
+                              ? p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + page]
+                              : fresh(lack[s] + static_cast<int>(page) - held);
+        if (entry >= 0) slot = entry * p.page_size + static_cast<int>(row);
+      }
+    }
+    p.positions[i] = position;
+    p.slots[i] = slot;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ norm, rotation, write
+
+constexpr int NR_THREADS = 256;
+constexpr int NR_UNROLL = 4;
+
+struct NormRopeParams {
+  const __nv_bfloat16 *q, *k, *v;                // v: or null (no cache)
+  const __nv_bfloat16 *q_gamma, *k_gamma;        // [D], or both null
+  __nv_bfloat16 *q_out, *k_out, *kv_cache;       // k_out or kv_cache
+  long long q_tok, k_tok, v_tok, qo_tok, ko_tok;  // elements from one token to the next
+  long long q_head, k_head, v_head, qo_head, ko_head;  // ... and from one head to the next
+  const int32_t *positions, *slots;
+  const float* cos_sin;  // [max_positions, rot]: cosines, then sines
+  int T, H, Hkv, rot, max_positions, interleaved, n_slots;
+  float eps;
+};
+
+// A lane holds eight elements of a head's row in two runs of four, at a and b: the two halves of four rotated pairs
+// (half-split: pair i is elements i and i + rot / 2) or four neighbouring pairs (interleaved), either way the pairs
+// 4 u .. 4 u + 3 of lane u; lanes past the rotated part hold eight elements that are only normed. So the rotation
+// needs no exchange between lanes, and each lane reads four cosines and four sines once for all heads of its token.
+// D / 8 lanes make a row, and a warp keeps NR_UNROLL rows a lane in flight. Everything is f32 from the load to the one
+// rounding of the result. Bound by HBM: each row is read once and written once.
+template <int D>
+__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const NormRopeParams p) {
+  constexpr int LANES = D / 8;            // lanes per row
+  constexpr int PER_PASS = 32 / LANES;    // rows per warp and pass
+  constexpr int ROWS = PER_PASS * NR_UNROLL;
+  const int lane = threadIdx.x & 31, u = lane % LANES, sub = lane / LANES;
+  const int heads = p.H + p.Hkv + (p.v != nullptr ? p.Hkv : 0);
+  const int chunks = (heads + ROWS - 1) / ROWS;
+  const long long items = static_cast<long long>(p.T) * chunks;
+  const bool rotated = u < p.rot / 8;
+  const int a = rotated ? (p.interleaved ? 8 * u : 4 * u) : p.rot + 8 * (u - p.rot / 8);
+  const int b = rotated && !p.interleaved ? p.rot / 2 + 4 * u : a + 4;
+  const int warps = gridDim.x * (NR_THREADS / 32);
+  for (long long item = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5); item < items; item += warps) {
+    const int tok = static_cast<int>(item / chunks), row0 = static_cast<int>(item % chunks) * ROWS + sub;
+    uint2 xa[NR_UNROLL], xb[NR_UNROLL];
+#pragma unroll
+    for (int i = 0; i < NR_UNROLL; ++i) {
+      const int r = row0 + i * PER_PASS;
+      const __nv_bfloat16* src = nullptr;
+      if (r < p.H) src = p.q + tok * p.q_tok + r * p.q_head;
+      else if (r < p.H + p.Hkv) src = p.k + tok * p.k_tok + (r - p.H) * p.k_head;
+      else if (r < heads) src = p.v + tok * p.v_tok + (r - p.H - p.Hkv) * p.v_head;
+      xa[i] = xb[i] = make_uint2(0, 0);
+      if (src != nullptr) {
+        xa[i] = *reinterpret_cast<const uint2*>(src + a);
+        xb[i] = *reinterpret_cast<const uint2*>(src + b);
+      }
+    }
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rotated) {
+      const int pos = min(max(p.positions[tok], 0), p.max_positions - 1);  // clamped, as a gather's index is
+      const float* table = p.cos_sin + static_cast<size_t>(pos) * p.rot;
+      c = *reinterpret_cast<const float4*>(table + 4 * u);
+      s = *reinterpret_cast<const float4*>(table + p.rot / 2 + 4 * u);
+    }
+    const int slot = p.slots != nullptr ? p.slots[tok] : -1;
+#pragma unroll
+    for (int i = 0; i < NR_UNROLL; ++i) {
+      const int r = row0 + i * PER_PASS;
+      const bool is_q = r < p.H, is_k = !is_q && r < p.H + p.Hkv;
+      uint2 oa = xa[i], ob = xb[i];
+      float x[8] = {bf16_lo(oa.x), bf16_hi(oa.x), bf16_lo(oa.y), bf16_hi(oa.y),
+                    bf16_lo(ob.x), bf16_hi(ob.x), bf16_lo(ob.y), bf16_hi(ob.y)};
+      if (p.q_gamma != nullptr) {  // (the same for every lane: the shuffles are convergent)
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        const float scale = rsqrtf(sum * (1.0f / D) + p.eps);
+        if (is_q || is_k) {
+          const __nv_bfloat16* g = is_q ? p.q_gamma : p.k_gamma;
+          const uint2 ga = __ldg(reinterpret_cast<const uint2*>(g + a)), gb = __ldg(reinterpret_cast<const uint2*>(g + b));
+          const float gv[8] = {bf16_lo(ga.x), bf16_hi(ga.x), bf16_lo(ga.y), bf16_hi(ga.y),
+                               bf16_lo(gb.x), bf16_hi(gb.x), bf16_lo(gb.y), bf16_hi(gb.y)};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] *= scale * gv[j];
+        }
+      }
+      if (is_q || is_k) {
+        if (rotated) {
+          const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float xe = p.interleaved ? x[2 * j] : x[j], xf = p.interleaved ? x[2 * j + 1] : x[j + 4];
+            const float ye = xe * cv[j] - xf * sv[j], yf = xe * sv[j] + xf * cv[j];
+            if (p.interleaved) x[2 * j] = ye, x[2 * j + 1] = yf;
+            else x[j] = ye, x[j + 4] = yf;
+          }
+        }
+        oa = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        ob = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+      }
+      __nv_bfloat16* dst = nullptr;
+      if (is_q) {
+        dst = p.q_out + tok * p.qo_tok + r * p.qo_head;
+      } else if (r < heads) {
+        const int h = is_k ? r - p.H : r - p.H - p.Hkv;
+        if (p.kv_cache == nullptr)
+          dst = p.k_out + tok * p.ko_tok + h * p.ko_head;
+        else if (slot >= 0 && slot < p.n_slots)
+          dst = p.kv_cache + ((static_cast<size_t>(slot) * p.Hkv + h) * 2 + (is_k ? 0 : 1)) * D;
+      }
+      if (dst != nullptr) {
+        *reinterpret_cast<uint2*>(dst + a) = oa;
+        *reinterpret_cast<uint2*>(dst + b) = ob;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ accepted path
+
+constexpr int COMMIT_THREADS = 256;
+constexpr int COMMIT_BATCH = 8;
+
+// A CTA moves one sequence's accepted rows, each thread a 16-byte column of them, in path order and COMMIT_BATCH rows
+// at a time: all loads of a batch before its stores. The path's nodes ascend, so node d's row never lies in front of
+// row d, no batch overwrites a row a later batch reads, and columns are independent: nothing is synchronised.
+__global__ void __launch_bounds__(COMMIT_THREADS)
+    rpa_commit_kernel(uint4* __restrict__ kv_cache, const int32_t* __restrict__ kv_lens,
+                      const int32_t* __restrict__ page_indices, const int32_t* __restrict__ cu_q_lens,
+                      const int32_t* __restrict__ paths, const int32_t* __restrict__ n_accepted, int P, int row_units,
+                      int page_size, int pages_per_seq, int num_pages, int32_t* __restrict__ out_lens) {
+  const int s = blockIdx.x, col = blockIdx.y * COMMIT_THREADS + threadIdx.x;
+  const int kv_len = kv_lens[s], q_len = max(cu_q_lens[s + 1] - cu_q_lens[s], 0), asked = n_accepted[s];
+  if (asked < 0) {  // nothing was drafted: every new token stays
+    if (col == 0) out_lens[s] = kv_len;
+    return;
+  }
+  const int ctx = max(kv_len - q_len, 0);
+  const int32_t* path = paths + static_cast<size_t>(s) * P;
+  const int32_t* table = page_indices + static_cast<size_t>(s) * pages_per_seq;
+  auto row = [&](int place) -> long long {  // 16-byte units from the cache's start, or -1: no such row
+    const int entry = place / page_size;
+    if (place < 0 || entry >= pages_per_seq) return -1;
+    const int page = table[entry];
+    if (page < 0 || page >= num_pages) return -1;
+    return (static_cast<long long>(page) * page_size + place % page_size) * row_units;
+  };
+  const int limit = min(asked, P);
+  int kept = 0, last = -1;
+  bool go = true;
+  for (int d0 = 0; d0 < limit && go; d0 += COMMIT_BATCH) {
+    uint4 data[COMMIT_BATCH];
+    long long to[COMMIT_BATCH];
+#pragma unroll
+    for (int i = 0; i < COMMIT_BATCH; ++i) {
+      to[i] = -1;
+      if (!go || d0 + i >= limit) continue;
+      const int node = path[d0 + i];
+      if (node <= last || node >= q_len) {  // not a path: it ends in front of this entry
+        go = false;
+        continue;
+      }
+      last = node, ++kept;
+      if (node == d0 + i || col >= row_units) continue;  // already where it belongs
+      const long long from = row(ctx + node);
+      const long long dst = row(ctx + d0 + i);
+      if (from < 0 || dst < 0) continue;
+      data[i] = kv_cache[from + col];
+      to[i] = dst + col;
+    }
+#pragma unroll
+    for (int i = 0; i < COMMIT_BATCH; ++i)
+      if (to[i] >= 0) kv_cache[to[i]] = data[i];
+  }
+  if (col == 0) out_lens[s] = ctx + kept;
+}
+
+}  // namespace tjx
+
+extern "C" {
+
+int tjx_rpa_plan(const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* pages_held, const int32_t* depths,
+                 int32_t* page_indices, const int32_t* free_pages, const int32_t* n_free, int free_capacity, int S, int T,
+                 int pages_per_seq, int page_size, int32_t* kv_lens, int32_t* cu_q_lens, int32_t* positions,
+                 int32_t* slots, int32_t* pages_held_out, int32_t* n_free_out, tjx_stream_t stream) {
+  using namespace tjx;
+  if (int rc = check_device()) return rc;
+  if (!ctx_lens || !q_lens || !page_indices || !n_free || !kv_lens || !cu_q_lens || !pages_held_out || !n_free_out ||
+      (T > 0 && (!positions || !slots)) || (free_capacity > 0 && !free_pages))
+    return fail(TJX_E_ARG, "an input or output pointer is null");
+  if (S <= 0 || T < 0 || pages_per_seq <= 0 || page_size <= 0 || free_capacity < 0)
+    return fail(TJX_E_ARG, "sizes must be positive");
+  if (S > PLAN_MAX_SEQS) return fail(TJX_E_LIMIT, "more than 8192 sequences");
+  if (static_cast<long long>(S) * pages_per_seq >= (1ll << 31))
+    return fail(TJX_E_LIMIT, "S * pages_per_seq must fit in int32");
+  if (T > (1 << 30)) return fail(TJX_E_LIMIT, "more than 2^30 tokens");
+  PlanParams p{};
+  p.ctx_lens = ctx_lens, p.q_lens = q_lens, p.held = pages_held, p.depths = depths;
+  p.page_indices = page_indices, p.free_pages = free_pages, p.n_free = n_free, p.free_capacity = free_capacity;
+  p.S = S, p.T = T, p.pages_per_seq = pages_per_seq, p.page_size = page_size;
+  p.kv_lens = kv_lens, p.cu_q_lens = cu_q_lens, p.positions = positions, p.slots = slots;
+  p.held_out = pages_held_out, p.n_free_out = n_free_out;
+  const size_t smem = 2 * static_cast<size_t>(S + 1) * sizeof(int);
+  static bool configured[64] = {};
+  int dev = 0;
+  TJX_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    TJX_CUDA(cudaFuncSetAttribute(rpa_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PLAN_MAX_SEQS + 1) * 4));
+    configured[dev & 63] = true;
+  }
+  const int grid = std::max(1, std::min((T + PLAN_THREADS - 1) / PLAN_THREADS, sm_count()));
+  rpa_plan_kernel<<<grid, PLAN_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(p);
+  TJX_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int tjx_norm_rope_bf16(const void* q, const void* k, const void* v, const int64_t* strides, const void* q_gamma,
+                       const void* k_gamma, const int32_t* positions, const float* cos_sin, const int32_t* slots,
+                       void* q_out, void* k_out, void* kv_cache, int T, int H, int Hkv, int D, int rot, int max_positions,
+                       int interleaved, int n_slots, float eps, tjx_stream_t stream) {
+  using namespace tjx;
+  if (int rc = check_device()) return rc;
+  if (!q || !k || !strides || !positions || (rot > 0 && !cos_sin) || !q_out) return fail(TJX_E_ARG, "an input or output pointer is null");
+  if ((q_gamma == nullptr) != (k_gamma == nullptr)) return fail(TJX_E_ARG, "q_gamma and k_gamma are given together or not at all");
+  const bool to_cache = kv_cache != nullptr;
+  if (to_cache ? (!v || !slots || n_slots <= 0) : (!k_out || v != nullptr || slots != nullptr))
+    return fail(TJX_E_ARG, "v, slots and kv_cache go together, or k_out alone");
+  if (T <= 0 || H <= 0 || Hkv <= 0 || max_positions <= 0) return fail(TJX_E_ARG, "sizes must be positive");
+  if (D != 64 && D != 128 && D != 256) return fail(TJX_E_ARG, "head dimension must be 64, 128 or 256");
+  if (rot < 0 || rot > D || rot % 8 != 0) return fail(TJX_E_ARG, "the rotated part is a multiple of 8, at most the head dimension");
+  if (!(eps >= 0.f)) return fail(TJX_E_ARG, "eps must not be negative");
+  const void* aligned8[] = {q, k, v, q_gamma, k_gamma, q_out, k_out, kv_cache};
+  for (const void* ptr : aligned8)
+    if (reinterpret_cast<uintptr_t>(ptr) & 7u) return fail(TJX_E_ARG, "bf16 operands must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(cos_sin) & 15u) return fail(TJX_E_ARG, "cos_sin must be 16-byte aligned");
+  for (int i = 0; i < 10; ++i)
+    if (strides[i] % 4 != 0 || strides[i] < 0) return fail(TJX_E_ARG, "strides must be multiples of 4 elements");
+  NormRopeParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.q_gamma = static_cast<const __nv_bfloat16*>(q_gamma), p.k_gamma = static_cast<const __nv_bfloat16*>(k_gamma);
+  p.q_out = static_cast<__nv_bfloat16*>(q_out), p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.kv_cache = static_cast<__nv_bfloat16*>(kv_cache);
+  p.q_tok = strides[0], p.q_head = strides[1], p.k_tok = strides[2], p.k_head = strides[3], p.v_tok = strides[4];
+  p.v_head = strides[5], p.qo_tok = strides[6], p.qo_head = strides[7], p.ko_tok = strides[8], p.ko_head = strides[9];
+  p.positions = positions, p.slots = slots, p.cos_sin = cos_sin;
+  p.T = T, p.H = H, p.Hkv = Hkv, p.rot = rot, p.max_positions = max_positions, p.interleaved = interleaved;
+  p.n_slots = n_slots, p.eps = eps;
+  const int rows = NR_UNROLL * 32 / (D / 8);
+  const int heads = H + Hkv * (to_cache ? 2 : 1);
+  const long long items = static_cast<long long>(T) * ((heads + rows - 1) / rows);
+  const int grid = static_cast<int>(std::min<long long>((items + NR_THREADS / 32 - 1) / (NR_THREADS / 32), sm_count() * 8ll));
+  auto kernel = D == 64 ? norm_rope_kernel<64> : D == 128 ? norm_rope_kernel<128> : norm_rope_kernel<256>;
+  kernel<<<grid, NR_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  TJX_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int tjx_rpa_commit_bf16(void* kv_cache, const int32_t* kv_lens, const int32_t* page_indices, const int32_t* cu_q_lens,
+                        const int32_t* paths, const int32_t* n_accepted, int32_t* out_lens, int S, int P, int Hkv, int D,
+                        int page_size, int pages_per_seq, int num_pages, tjx_stream_t stream) {
+  using namespace tjx;
+  if (int rc = check_device()) return rc;
+  if (!kv_cache || !kv_lens || !page_indices || !cu_q_lens || !paths || !n_accepted || !out_lens)
+    return fail(TJX_E_ARG, "an input or output pointer is null");
+  if (S <= 0 || P <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || pages_per_seq <= 0 || num_pages <= 0)
+    return fail(TJX_E_ARG, "sizes must be positive");
+  if (D % 8 != 0) return fail(TJX_E_ARG, "head dimension must be a multiple of 8");
+  if (reinterpret_cast<uintptr_t>(kv_cache) & 15u) return fail(TJX_E_ARG, "kv_cache must be 16-byte aligned");
+  if (static_cast<long long>(Hkv) * D > (1ll << 24)) return fail(TJX_E_LIMIT, "Hkv * D is too large");
+  const int row_units = Hkv * 2 * D * 2 / 16;
+  const dim3 grid(S, (row_units + COMMIT_THREADS - 1) / COMMIT_THREADS);
+  rpa_commit_kernel<<<grid, COMMIT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<uint4*>(kv_cache), kv_lens, page_indices, cu_q_lens, paths, n_accepted, P, row_units, page_size,
+      pages_per_seq, num_pages, out_lens);
+  TJX_CUDA(cudaGetLastError());
+  return 0;
+}
+
+}  // extern "C"

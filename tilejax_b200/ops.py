@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import hashlib
 from functools import lru_cache
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -629,6 +630,235 @@ def ragged_paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
             _ptr(distribution), _ptr(out), T, S, H, Hkv, D, page_size, pps, num_pages, float(sm_scale),
             ctypes.c_void_p(ws_ptr), need, _stream()))
     return out, kv_cache
+
+
+# ------------------------------------------------------------------------------------------ a step over drafted tokens
+
+
+def _int32_vectors(**tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.dim() != 1:
+            raise ValueError(f"{name} must be an int32 vector")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of the one meets that of the other."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    def end(t):
+        return t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
+class RpaStep(NamedTuple):
+    """What `rpa_plan` makes of a step: everything the other `rpa_*` operators take beside the data."""
+
+    kv_lens: torch.Tensor      # (S,) cache positions of each sequence, the new tokens included
+    cu_q_lens: torch.Tensor    # (S + 1,) first token of each sequence, then their number
+    positions: torch.Tensor    # (T,) position of each token in its text, what its rotation goes by
+    slots: torch.Tensor        # (T,) cache row (page * page_size + row) of each token, -1 where it has none
+    pages_held: torch.Tensor   # (S,) pages of each sequence
+    n_free: torch.Tensor       # (2,) pages left on the free stack, pages that were missing
+
+
+def rpa_plan(ctx_lens: torch.Tensor, q_lens: torch.Tensor, page_indices: torch.Tensor, free_pages: torch.Tensor,
+             n_free: torch.Tensor, page_size: int, tokens: int, pages_held: torch.Tensor | None = None,
+             depths: torch.Tensor | None = None, out: RpaStep | None = None) -> RpaStep:
+    """Block tables and slot map of a step, made on the GPU from the requests' lengths in one launch: sequence s has
+    ctx_lens[s] positions cached on pages_held[s] pages (just enough if not given) and brings q_lens[s] new tokens, in
+    all at most `tokens` rows. The pages it lacks come off the top of the stack free_pages[: n_free[0]], sequence after
+    sequence, and are entered in page_indices (S * pages_per_seq,) IN PLACE behind those it holds, -1 where the stack
+    is empty. `depths` (tokens,) gives drafted tokens their depth in the tree: the token's position is then ctx_lens[s]
+    plus its depth, while its slot stays that of its index. `out` is written instead of new tensors; it may not overlap
+    the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into ctx_lens)."""
+    inputs = [t for t in (ctx_lens, q_lens, page_indices, free_pages, n_free, pages_held, depths) if t is not None]
+    _int32_vectors(ctx_lens=ctx_lens, q_lens=q_lens, page_indices=page_indices, free_pages=free_pages, n_free=n_free)
+    S, T = ctx_lens.shape[0], int(tokens)
+    if S == 0 or q_lens.shape[0] != S or page_indices.shape[0] == 0 or page_indices.shape[0] % S:
+        raise ValueError("ctx_lens and q_lens are (S,), page_indices (S * pages_per_seq,)")
+    if n_free.shape[0] < 1:
+        raise ValueError("n_free holds the number of free pages")
+    if pages_held is not None and (pages_held.shape != (S,) or pages_held.dtype != torch.int32):
+        raise ValueError("pages_held is int32 (S,)")
+    if depths is not None and (depths.shape != (T,) or depths.dtype != torch.int32):
+        raise ValueError("depths is int32 (tokens,)")
+    if T < 0 or page_size <= 0:
+        raise ValueError("page_size must be positive and tokens not negative")
+    device = _need_cuda(*inputs)
+    if out is None:
+        out = RpaStep(*torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device).split([S, S + 1, T, T, S, 2]))
+    else:
+        _need_cuda(ctx_lens, *out)
+        if [tuple(t.shape) for t in out] != [(S,), (S + 1,), (T,), (T,), (S,), (2,)] or any(t.dtype != torch.int32 for t in out):
+            raise ValueError("out is a step of other sizes")
+        if any(_overlap(a, b) for a in out for b in inputs):
+            raise ValueError("out overlaps an input")
+    with torch.cuda.device(device):
+        check(library().tjx_rpa_plan(_ptr(ctx_lens), _ptr(q_lens), _ptr(pages_held), _ptr(depths), _ptr(page_indices),
+                                     _ptr(free_pages), _ptr(n_free), free_pages.shape[0], S, T,
+                                     page_indices.shape[0] // S, page_size, *map(_ptr, out), _stream()))
+    return out
+
+
+def _heads(name: str, t: torch.Tensor, tokens: int, heads: int | None, D: int) -> None:
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[0] != tokens or t.shape[2] != D or \
+            (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be bfloat16 ({tokens}, {'heads' if heads is None else heads}, {D})")
+    if t.stride(2) != 1 or t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
+        raise ValueError(f"{name}'s last dimension must be dense, its strides multiples of 4 elements, its data 8-byte aligned")
+
+
+def _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, kv_cache, slots, eps, interleaved):
+    if q.dim() != 3:
+        raise ValueError("q is (T, H, D)")
+    T, H, D = q.shape
+    Hkv = k.shape[1] if k.dim() == 3 else 0
+    _heads("q", q, T, None, D)
+    _heads("k", k, T, None, D)
+    if (q_gamma is None) != (k_gamma is None):
+        raise ValueError("q_gamma and k_gamma are given together or not at all")
+    for g in (q_gamma, k_gamma):
+        if g is not None and (g.shape != (D,) or g.dtype != torch.bfloat16 or not g.is_contiguous() or g.data_ptr() % 8):
+            raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
+    if positions.shape != (T,) or positions.dtype != torch.int32:
+        raise ValueError("positions is int32 (T,)")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] > D or cos_sin.shape[1] % 8 \
+            or cos_sin.shape[0] == 0 or cos_sin.data_ptr() % 16:
+        raise ValueError("cos_sin is float32 (max_positions, rot), rot a multiple of 8 up to the head dimension, 16-byte aligned")
+    device = _need_cuda(positions, cos_sin, *(t for t in (q_gamma, k_gamma, slots) if t is not None))
+    used = [t for t in (q, k, v) if t is not None]
+    if any(t.device != device for t in used):
+        raise ValueError("all tensors must be on the same device")
+    if q_out is None:
+        q_out = torch.empty((T, H, D), dtype=q.dtype, device=device)
+    elif q_out is not q:
+        _heads("the queries' output", q_out, T, H, D)
+        if q_out.device != device or any(_overlap(q_out, t) for t in used if not _same(q_out, q)):
+            raise ValueError("the queries' output is q itself or memory of its own, on q's device")
+    if kv_cache is None:
+        if k_out is None:
+            k_out = torch.empty((T, Hkv, D), dtype=k.dtype, device=device)
+        elif k_out is not k:
+            _heads("the keys' output", k_out, T, Hkv, D)
+            if k_out.device != device or any(_overlap(k_out, t) for t in (*used, q_out) if not _same(k_out, k)):
+                raise ValueError("the keys' output is k itself or memory of its own, on k's device")
+    elif any(_overlap(kv_cache, t) for t in (*used, q_out)):
+        raise ValueError("the cache overlaps an operand")
+    if T == 0:
+        return q_out, k_out
+    strides = (ctypes.c_int64 * 10)(*(x for t in (q, k, k if v is None else v, q_out, k if k_out is None else k_out)
+                                      for x in t.stride()[:2]))
+    with torch.cuda.device(device):
+        check(library().tjx_norm_rope_bf16(
+            _ptr(q), _ptr(k), _ptr(v), strides, _ptr(q_gamma), _ptr(k_gamma), _ptr(positions), _ptr(cos_sin), _ptr(slots),
+            _ptr(q_out), _ptr(k_out), _ptr(kv_cache), T, H, Hkv, D, cos_sin.shape[1], cos_sin.shape[0], int(interleaved),
+            0 if kv_cache is None else kv_cache.shape[0] * kv_cache.shape[1], float(eps), _stream()))
+    return q_out, k_out
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None,
+                 positions: torch.Tensor, cos_sin: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
+                 out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of q (T, H, D) and k (T, Hkv, D) and its rotation by the token's position, in one pass:
+    x * rsqrt(mean(x^2) + eps) * gamma (no norm where the gammas are None), then pair i of the first `rot` elements
+    turned by the angle whose cosine and sine are cos_sin[positions[t], i] and [.., rot / 2 + i] (float32
+    (max_positions, rot); positions past the table are clamped to it). Pair i is elements i and i + rot / 2, or 2 i and
+    2 i + 1 if `interleaved`. q and k may be views of one projection's output: any token and head strides that are
+    multiples of 4. Returns (q', k'); out=(q, k) updates in place. D 64, 128 or 256."""
+    q_out, k_out = out if out is not None else (None, None)
+    return _norm_rope(q, k, None, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, None, None, eps, interleaved)
+
+
+def rpa_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gamma: torch.Tensor | None,
+                        k_gamma: torch.Tensor | None, positions: torch.Tensor, cos_sin: torch.Tensor,
+                        kv_cache: torch.Tensor, slots: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
+                        out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`qk_norm_rope` with the cache write in the same pass: the turned key and the value of token t go to row slots[t]
+    (page * page_size + row, as `rpa_plan` gives it; out of range: not written; no slot twice) of the cache
+    (pages, page_size, Hkv, 2, D), IN PLACE. Returns (q', the cache); `out=q` updates the queries in place."""
+    if kv_cache.dim() != 5 or kv_cache.shape[3] != 2 or kv_cache.dtype != torch.bfloat16 or not kv_cache.is_contiguous() \
+            or kv_cache.numel() == 0:
+        raise ValueError("the cache is (pages, page_size, Hkv, 2, D) bfloat16: each head's key and value side by side")
+    if q.dim() != 3 or k.shape != v.shape or k.shape[1:] != (kv_cache.shape[2], kv_cache.shape[4]):
+        raise ValueError("q is (T, H, D), k and v (T, Hkv, D) with the cache's Hkv and D")
+    if kv_cache.shape[0] * kv_cache.shape[1] >= 1 << 31:
+        raise ValueError("the cache's rows must fit in int32")
+    if slots.shape != (q.shape[0],) or slots.dtype != torch.int32 or slots.device != kv_cache.device:
+        raise ValueError("slots is int32 (T,), on the cache's device")
+    _heads("v", v, q.shape[0], k.shape[1], q.shape[2])
+    q_out, _ = _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, out, None, kv_cache, slots, eps, interleaved)
+    return q_out, kv_cache
+
+
+def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor,
+                       cu_q_lens: torch.Tensor, tree_mask: torch.Tensor, distribution: torch.Tensor,
+                       sm_scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`rpa_decode` for sequences that bring several drafted tokens each: sequence s < distribution[0] has the tokens
+    cu_q_lens[s] .. cu_q_lens[s + 1] - 1 of q (T, H, D), written to the cache behind the others of its kv_lens[s]
+    positions. Token t attends to every position before its sequence's new tokens and to those new tokens j whose bit
+    (bit j % 32 of word j // 32) is set in tree_mask[t], int32 (T, words): its ancestors and itself. Their rows become
+    the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
+    the sequences from distribution[0] on. `out=q` updates in place."""
+    num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
+    if q.dim() != 3 or q.shape[2] != D or q.dtype != torch.bfloat16:
+        raise ValueError("q is (T, H, D) bfloat16")
+    T, H, _ = q.shape
+    if cu_q_lens.shape != (S + 1,) or distribution.shape != (3,) or cu_q_lens.dtype != torch.int32 \
+            or distribution.dtype != torch.int32:
+        raise ValueError("cu_q_lens is int32 (S + 1,), distribution int32 (3,)")
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.shape[1] == 0 or tree_mask.dtype != torch.int32:
+        raise ValueError("tree_mask is int32 (T, words), 32 new tokens a word")
+    device = _need_cuda(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
+        raise ValueError("out must look like q")
+    elif out.data_ptr() != q.data_ptr() and _overlap(out, q):
+        raise ValueError("out is q itself or memory of its own")
+    if T == 0:
+        return out
+    with torch.cuda.device(device):
+        need = int(library().tjx_rpa_tree_attention_workspace_bytes(T, S, H, Hkv))
+        ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
+        ws_ptr = (ws.data_ptr() + 255) & ~255
+        check(library().tjx_rpa_tree_attention_bf16(
+            _ptr(q), _ptr(out), _ptr(kv_cache), _ptr(kv_lens), _ptr(page_indices), _ptr(cu_q_lens), _ptr(tree_mask),
+            _ptr(distribution), T, S, H, Hkv, D, tree_mask.shape[1], page_size, pps, num_pages, float(sm_scale),
+            ctypes.c_void_p(ws_ptr), need, _stream()))
+    return out
+
+
+def rpa_commit(kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor, cu_q_lens: torch.Tensor,
+               paths: torch.Tensor, n_accepted: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Keeps the accepted path of each sequence's drafted tokens: the cache rows of its nodes paths[s, : n_accepted[s]]
+    (int32 (S, P), ascending indices among the sequence's new tokens) move together behind the positions before them,
+    IN PLACE, and the sequence's length becomes those positions and the accepted tokens; n_accepted[s] < 0 keeps all
+    its tokens. A path ends in front of an entry that does not ascend or is no new token. Returns the lengths, int32
+    (S,), `out` if given (not kv_lens itself)."""
+    num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
+    if cu_q_lens.shape != (S + 1,) or cu_q_lens.dtype != torch.int32:
+        raise ValueError("cu_q_lens is int32 (S + 1,)")
+    if paths.dim() != 2 or paths.shape[0] != S or paths.shape[1] == 0 or paths.dtype != torch.int32 \
+            or n_accepted.shape != (S,) or n_accepted.dtype != torch.int32:
+        raise ValueError("paths is int32 (S, P), n_accepted int32 (S,)")
+    device = _need_cuda(kv_cache, kv_lens, page_indices, cu_q_lens, paths, n_accepted)
+    if out is None:
+        out = torch.empty(S, dtype=torch.int32, device=device)
+    elif out.shape != (S,) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != device:
+        raise ValueError("out is int32 (S,), on the cache's device")
+    elif any(_overlap(out, t) for t in (kv_lens, page_indices, cu_q_lens, paths, n_accepted)):
+        raise ValueError("out overlaps an input")
+    with torch.cuda.device(device):
+        check(library().tjx_rpa_commit_bf16(_ptr(kv_cache), _ptr(kv_lens), _ptr(page_indices), _ptr(cu_q_lens), _ptr(paths),
+                                            _ptr(n_accepted), _ptr(out), S, paths.shape[1], Hkv, D, page_size, pps,
+                                            num_pages, _stream()))
+    return out
 
 
 def paged_gqa_decode_static(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
