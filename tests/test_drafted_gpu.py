@@ -258,6 +258,46 @@ def test_tree_attention_at_its_edges(kw, case):
     check_tree(tree_case(*case, **kw))
 
 
+def tree_attention_on_the_gpu(inp, sm_scale):
+    """oracle.tree_attention_f64 in torch's float64, for sizes NumPy takes long over (no hidden NaN)."""
+    q, cache = inp["q"].double(), inp["kv_cache"]
+    pages, page, hkv, _, D = cache.shape
+    S = inp["kv_lens"].shape[0]
+    table = inp["page_indices"].view(S, -1)
+    cu, lens = inp["cu_q_lens"].tolist(), inp["kv_lens"].tolist()
+    out, size = q.clone(), torch.zeros_like(q)
+    for s in range(S):
+        n, length = cu[s + 1] - cu[s], lens[s]
+        kv = cache[table[s, : -(-length // page)].long()].reshape(-1, hkv, 2, D)[:length].double()
+        bits = (inp["tree_mask"][cu[s] : cu[s + 1], :, None] >> torch.arange(32, device="cuda", dtype=torch.int32)) & 1
+        sees = torch.cat([torch.ones(n, length - n, device="cuda", dtype=torch.bool), bits.reshape(n, -1)[:, :n].bool()], 1)
+        rows = q[cu[s] : cu[s + 1]].view(n, hkv, -1, D)
+        z = torch.einsum("nhgd,phd->nhgp", rows, kv[:, :, 0]) * sm_scale
+        w = z.masked_fill(~sees[:, None, None], -float("inf")).softmax(-1)
+        out[cu[s] : cu[s + 1]] = torch.einsum("nhgp,phd->nhgd", w, kv[:, :, 1]).reshape(n, -1, D)
+        size[cu[s] : cu[s + 1]] = torch.einsum("nhgp,phd->nhgd", w, kv[:, :, 1].abs()).reshape(n, -1, D)
+    return out.cpu().numpy(), size.cpu().numpy()
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize(("heads", "kv_heads", "page", "seqs", "nodes", "ctx"), [
+    (28, 4, 48, 13, 25, 2749),   # units of one and of two row tiles, many in one CTA's run, others over many CTAs
+    (8, 2, 16, 40, 9, 600),      # small units: several in every run
+    (16, 2, 128, 3, 64, 20000),  # every unit over many CTAs
+])
+def test_runs_of_many_units_and_units_of_many_runs(heads, kv_heads, page, seqs, nodes, ctx, seed):
+    rng = np.random.default_rng(seed)
+    q_lens = [int(n) for n in rng.integers(1, nodes + 1, seqs)]
+    kv_lens = [n + int(c) for n, c in zip(q_lens, rng.integers(0, ctx, seqs))]
+    dev = {k: to_device(v) for k, v in tree_case(q_lens, kv_lens, heads, kv_heads, page, seed=seed, scale=2.0, poison=False).items()}
+    want, size = tree_attention_on_the_gpu(dev, 128**-0.5)
+    first = ops.rpa_tree_attention(**dev, sm_scale=128**-0.5)
+    close(to_host(first), want, size, 2.0**-8 + 2.0**-11)
+    for _ in range(20):  # the same bits every time
+        assert torch.equal(ops.rpa_tree_attention(**dev, sm_scale=128**-0.5).view(torch.int16), first.view(torch.int16))
+    assert ops.device_status() == 0
+
+
 def test_a_longer_tree_than_its_cache_and_lengths_past_the_table():
     inp = tree_case([6, 4], [20, 30], 8, 2, 16)
     inp["kv_lens"][0] = 4          # four positions for six nodes: the first two are in no cache row

@@ -3,6 +3,24 @@
 // prefix and those of its own sequence that its mask names (its ancestors in the tree, and itself).
 //   o[t, h] = sum_p softmax_p(sm_scale q[t, h] . k[p, h / group]) v[p, h / group]
 // over the positions p < kv_len - q_len and the nodes j (position kv_len - q_len + j) with bit j of tree_mask[t] set.
+//
+// The rows (node, query head) that share a KV head share its cache, so a position costs 512 bytes of HBM and, at 128
+// rows of tensor work however few are used, 65 k multiply-adds: 11.6 ns of one SM's share of the memory rate against
+// 5.8 of its tensor rate. So one kernel serves one node and many: whole 128-row tcgen05 tiles, padded.
+//
+// A unit is (sequence, KV head, up to 256 rows): its rows make one tile of 128, or two that share every K / V block of
+// 64 positions. The blocks of all units, in order, are cut into equal runs, one for each CTA: a CTA walks the end of
+// one unit, whole units, and the beginning of another, and what it has of a unit that others share is a partial result
+// (running maximum, sum, unnormalised rows) that tree_join_kernel joins in order. One persistent CTA per SM:
+//
+//   warp 0      producer: TMA loads of Q (a buffer per row tile), K and V blocks (boxes of at most a page) into rings
+//   warp 1      MMA issuer: S = Q K^T of two jobs ahead of O += P V, P read from TMEM
+//   warps 2-5   softmax of the even jobs, warps 6-9 of the odd ones (a thread owns a row)
+//
+// A job is (row tile, block). With two row tiles the jobs of a block are its two tiles; with one tile they are
+// successive blocks, so the two softmax groups each keep a running maximum, sum and output over half of the blocks and
+// join them in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
+// the scores), so that the next scores are made while it works, and 128 columns of output.
 #include <algorithm>
 
 #include "tjx_host.cuh"
@@ -13,7 +31,15 @@
 namespace tjx {
 
 constexpr int TR_D = 128;
+constexpr int TR_ROWS = 128;   // rows of a tile
+constexpr int TR_BLOCK = 64;   // positions of a block
+constexpr int TR_K_STAGES = 4;
+constexpr int TR_V_STAGES = 5;  // a V block is held longer: until its probabilities are made
+constexpr int TR_THREADS = 320;
 constexpr float TR_LOG2E = 1.4426950408889634f;
+constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a row that has seen nothing
+constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
+constexpr int TR_MIN_SHARE = 4;       // blocks of a CTA's run, at least
 
 struct TreeParams {
   const __nv_bfloat16* q;
@@ -21,93 +47,686 @@ struct TreeParams {
   const __nv_bfloat16* kv_cache;
   const int32_t *kv_lens, *page_indices, *cu_q_lens, *tree_mask, *distribution;
   int T, S, H, Hkv, group, page_size, pages_per_seq, num_pages, words;
+  int tile_nodes;  // nodes of a row tile: 128 / group
+  int box_rows;    // positions of one TMA box: the largest power of two that divides the page size, at most 64
   float scale_log2e;
+  int part_rows;     // rows of a partial result
+  float* part_o;     // [2 CTAs][part_rows][128]
+  float2* part_ml;   // [2 CTAs][part_rows]: running maximum (log2 units) and sum
+  int4* joins;       // [CTAs]: the unit that starts in CTA c and ends in a later one: first token, nodes, KV head, last CTA
+  int* status;
 };
 
-// A warp per (token, query head): 32 positions at a time, a lane per position for the scores (q in shared memory, the
-// lane reads its key's row), then four of the 128 output dimensions per lane. Positions the mask hides are skipped, so
-// what they hold does not matter.
-__global__ void __launch_bounds__(128) tree_simple_kernel(const TreeParams p) {
-  __shared__ float q_sh[4][TR_D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (item >= static_cast<long long>(p.T) * p.H) return;
-  const int t = static_cast<int>(item / p.H), h = static_cast<int>(item % p.H), hk = h / p.group;
-  const uint2 raw = reinterpret_cast<const uint2*>(p.q + item * TR_D)[lane];
-  const int seqs = min(max(p.distribution[0], 0), p.S);
-  int lo = 0, hi = seqs;  // the sequence of token t: cu_q_lens[lo] <= t < cu_q_lens[lo + 1]
-  const bool covered = seqs > 0 && t >= p.cu_q_lens[0] && t < p.cu_q_lens[seqs];
-  uint2* dst = reinterpret_cast<uint2*>(p.out + item * TR_D) + lane;
-  if (!covered) {
-    if (p.out != p.q) *dst = raw;
-    return;
+struct TreeSmem {
+  static constexpr int Q_BYTES = TR_ROWS * TR_D * 2;   // two halves of 64 columns
+  static constexpr int KV_BYTES = TR_BLOCK * TR_D * 2;
+  static constexpr int Q_OFF = 0;  // two buffers
+  static constexpr int K_OFF = 2 * Q_BYTES;
+  static constexpr int V_OFF = K_OFF + TR_K_STAGES * KV_BYTES;
+  static constexpr int STAT_OFF = V_OFF + TR_V_STAGES * KV_BYTES;  // float2[2][128]: maximum and sum of each group's rows
+  static constexpr int BAD_OFF = STAT_OFF + 2 * TR_ROWS * 8;       // uint32[2 groups][2][4]: rows of V that are not finite
+  static constexpr int SCAN_OFF = BAD_OFF + 64;                    // long long[10], and where this CTA starts
+  static constexpr int BAR_OFF = SCAN_OFF + 160;
+  static constexpr int TOTAL = BAR_OFF + 512 + 1024;
+};
+static_assert(TreeSmem::TOTAL <= 232448, "shared memory of one CTA");
+
+// One sequence's sizes, clamped to what the arrays hold.
+struct TreeSeq {
+  int tok0, q_len, ctx, end, blocks, pairs;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
+  TreeSeq r;
+  const int c0 = p.cu_q_lens[s], c1 = p.cu_q_lens[s + 1], len = p.kv_lens[s];
+  r.tok0 = min(max(c0, 0), p.T);
+  r.q_len = max(min(c1, p.T) - r.tok0, 0);
+  r.end = min(max(len, 0), p.pages_per_seq * p.page_size);  // positions to walk
+  r.ctx = len < 0 ? -r.q_len : len - r.q_len;               // position of node 0
+  r.blocks = max((r.end + TR_BLOCK - 1) / TR_BLOCK, 1);     // (one where there is nothing: its rows become zero)
+  r.pairs = (r.q_len + 2 * p.tile_nodes - 1) / (2 * p.tile_nodes);
+  return r;
+}
+
+// A CTA's walk over its run of blocks: the same in every role.
+struct TreePortion {
+  int s, tok, nodes;     // first token and nodes of the unit
+  int hk, ctx, end;
+  int node0;             // (first node's index in its sequence)
+  int j0, j1;            // blocks of the unit
+  bool whole, starts;    // all of the unit's blocks; its first block among them
+  int jobs;              // softmax jobs: blocks, twice as many with two row tiles
+  bool two;              // two row tiles
+  long long after;       // blocks of the unit behind this portion
+};
+struct TreeWalk {
+  int s, hk, pr, j;
+  long long left;
+  TreeSeq q;
+  // From block `off` of sequence s on.
+  __device__ __forceinline__ void start(const TreeParams& p, int s_, long long off, long long count) {
+    s = s_, left = count;
+    hk = pr = j = 0;
+    if (left <= 0) return;
+    load(p);
+    const int unit = static_cast<int>(off / q.blocks);
+    j = static_cast<int>(off % q.blocks);
+    hk = unit / q.pairs, pr = unit % q.pairs;
   }
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q_lens[mid] <= t) lo = mid; else hi = mid;
+  __device__ __forceinline__ void load(const TreeParams& p) {  // by whole warps: the same values, and said to be so
+    q = tree_seq(p, s);
+    q.tok0 = __shfl_sync(0xFFFFFFFFu, q.tok0, 0), q.q_len = __shfl_sync(0xFFFFFFFFu, q.q_len, 0);
+    q.ctx = __shfl_sync(0xFFFFFFFFu, q.ctx, 0), q.end = __shfl_sync(0xFFFFFFFFu, q.end, 0);
+    q.blocks = __shfl_sync(0xFFFFFFFFu, q.blocks, 0), q.pairs = __shfl_sync(0xFFFFFFFFu, q.pairs, 0);
   }
-  const int s = lo, q_len = p.cu_q_lens[s + 1] - p.cu_q_lens[s];
-  const long long ctx = static_cast<long long>(p.kv_lens[s]) - q_len;
-  const int end = static_cast<int>(min(static_cast<long long>(max(p.kv_lens[s], 0)),
-                                       static_cast<long long>(p.pages_per_seq) * p.page_size));
-  q_sh[warp][4 * lane] = bf16_lo(raw.x) * p.scale_log2e, q_sh[warp][4 * lane + 1] = bf16_hi(raw.x) * p.scale_log2e;
-  q_sh[warp][4 * lane + 2] = bf16_lo(raw.y) * p.scale_log2e, q_sh[warp][4 * lane + 3] = bf16_hi(raw.y) * p.scale_log2e;
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < end; p0 += 32) {
-    const int pos = p0 + lane;
-    bool sees = pos < end;
-    if (sees && pos >= ctx) {
-      const long long node = pos - ctx;
-      sees = node < 32ll * p.words && ((p.tree_mask[static_cast<size_t>(t) * p.words + node / 32] >> (node % 32)) & 1);
-    }
-    float score = 0.f;
-    long long row = 0;
-    if (pos < end) {
-      const int page = min(max(p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + pos / p.page_size], 0), p.num_pages - 1);
-      row = ((static_cast<long long>(page) * p.page_size + pos % p.page_size) * p.Hkv + hk) * 2 * TR_D;
-    }
-    if (sees) {
-      const uint4* k = reinterpret_cast<const uint4*>(p.kv_cache + row);
-#pragma unroll 4
-      for (int u = 0; u < TR_D / 8; ++u) {
-        const uint4 x = k[u];
-        const float* qv = &q_sh[warp][8 * u];
-        score += qv[0] * bf16_lo(x.x) + qv[1] * bf16_hi(x.x) + qv[2] * bf16_lo(x.y) + qv[3] * bf16_hi(x.y) +
-                 qv[4] * bf16_lo(x.z) + qv[5] * bf16_hi(x.z) + qv[6] * bf16_lo(x.w) + qv[7] * bf16_hi(x.w);
+  __device__ __forceinline__ bool next(const TreeParams& p, TreePortion& o) {
+    if (left <= 0) return false;
+    const int take = static_cast<int>(min(static_cast<long long>(q.blocks - j), left));
+    o.s = s, o.hk = hk, o.ctx = q.ctx, o.end = q.end;
+    o.node0 = pr * 2 * p.tile_nodes;
+    o.tok = q.tok0 + o.node0;
+    o.nodes = min(q.q_len - o.node0, 2 * p.tile_nodes);
+    o.two = o.nodes > p.tile_nodes;
+    o.j0 = j, o.j1 = j + take;
+    o.starts = j == 0, o.whole = o.starts && o.j1 == q.blocks;
+    o.after = q.blocks - o.j1;
+    o.jobs = o.two ? 2 * take : take;
+    left -= take, j += take;
+    if (j == q.blocks) {
+      j = 0;
+      if (++pr == q.pairs) {
+        pr = 0;
+        if (++hk == p.Hkv) {
+          hk = 0;
+          if (left > 0) {
+            do ++s, load(p); while (q.pairs == 0);  // (blocks are left, so a sequence with some follows)
+          }
+        }
       }
     }
-    const unsigned seen = __ballot_sync(0xFFFFFFFFu, sees);
-    if (seen == 0) continue;
-    float mx = sees ? score : -INFINITY;
+    return true;
+  }
+};
+
+// 32 positions from `pos` on as a row sees them: its mask's bits from node pos - ctx on, ones before the first node,
+// zeros past the mask's words and from `end` on.
+__device__ __forceinline__ uint32_t tree_bits(const int32_t* mask, int words, int pos, int ctx, int end) {
+  uint32_t bits = 0xFFFFFFFFu;
+  if (pos + 32 > ctx) {
+    const int o = pos - ctx, w = o >> 5, shift = o & 31;  // (arithmetic shift: w = -1 or less before the nodes)
+    const uint32_t lo = w < 0 ? 0xFFFFFFFFu : w < words ? static_cast<uint32_t>(mask[w]) : 0u;
+    const uint32_t hi = w + 1 < 0 ? 0xFFFFFFFFu : w + 1 < words ? static_cast<uint32_t>(mask[w + 1]) : 0u;
+    bits = __funnelshift_r(lo, hi, shift);
+  }
+  const int valid = end - pos;
+  return valid >= 32 ? bits : valid <= 0 ? 0u : bits & ((1u << valid) - 1u);
+}
+
+__device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
+  return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+}
+
+__global__ void __launch_bounds__(TR_THREADS, 1)
+    tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const TreeParams p) {
+  using L = TreeSmem;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar = base + L::BAR_OFF;
+  auto q_full = [&](int b) { return bar + 8u * b; };
+  auto q_empty = [&](int b) { return bar + 8u * (2 + b); };
+  auto s_full = [&](int t, int b) { return bar + 8u * (4 + 2 * t + b); };
+  auto p_ready = [&](int t, int b) { return bar + 8u * (8 + 2 * t + b); };
+  auto o_done = [&](int t, int b) { return bar + 8u * (12 + 2 * t + b); };
+  auto v_seen = [&](int t) { return bar + 8u * (16 + t); };  // a group's warps have looked at a V block
+  const uint32_t v_seen_both = bar + 8u * 18;
+  const uint32_t stats_ready = bar + 8u * 19, outputs_read = bar + 8u * 20;
+  constexpr int RING = 21;
+  auto k_full = [&](int i) { return bar + 8u * (RING + i); };
+  auto k_empty = [&](int i) { return bar + 8u * (RING + TR_K_STAGES + i); };
+  auto v_full = [&](int i) { return bar + 8u * (RING + 2 * TR_K_STAGES + i); };
+  auto v_empty = [&](int i) { return bar + 8u * (RING + 2 * TR_K_STAGES + TR_V_STAGES + i); };
+  constexpr int N_BARS = RING + 2 * TR_K_STAGES + 2 * TR_V_STAGES;
+  volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(base_ptr + L::BAR_OFF + 8 * N_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + L::BAR_OFF + 8 * N_BARS + 8);
+  volatile long long* scan = reinterpret_cast<volatile long long*>(base_ptr + L::SCAN_OFF);
+  float2* stats = reinterpret_cast<float2*>(base_ptr + L::STAT_OFF);
+  volatile uint32_t* bad_rows = reinterpret_cast<volatile uint32_t*>(base_ptr + L::BAD_OFF);
+
+  const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < N_BARS; ++i) {
+      // p_ready, v_seen: the warps of a group; the next three: of both
+      const int arrivals = (i >= 8 && i < 12) || i == 16 || i == 17 ? 4 : i >= 18 && i < RING ? 8 : 1;
+      mbar_init(bar + 8u * i, arrivals);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_kv);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_holder)), 512);
+    tmem_relinquish();
+  }
+  // All blocks counted, and where this CTA's run starts: a thread takes consecutive sequences, the thread that has the
+  // run's first block finds its sequence.
+  const int seqs = min(max(p.distribution[0], 0), p.S);
+  const int per_thread = (seqs + TR_THREADS - 1) / TR_THREADS;
+  auto blocks_of = [&](int s) {
+    const TreeSeq q = tree_seq(p, s);
+    return static_cast<long long>(q.blocks) * q.pairs * p.Hkv;
+  };
+  const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, seqs), s_hi = min(s_lo + per_thread, seqs);
+  long long mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) mine += blocks_of(s);
+  long long upto = mine;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-    const float m_new = fmaxf(m, mx), alpha = ex2(m - m_new);
-    const float e = sees ? ex2(score - m_new) : 0.f;
-    m = m_new;
-    float sum = e;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += y;
+  }
+  if (lane == 31) scan[warp] = upto;
+  __syncthreads();
+  long long total = 0;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    l = l * alpha + sum;
+  for (int w = 0; w < TR_THREADS / 32; ++w) {
+    if (w == warp) upto += total;
+    total += scan[w];
+  }
+  const long long share = max((total + gridDim.x - 1) / static_cast<long long>(gridDim.x), static_cast<long long>(TR_MIN_SHARE));
+  const long long first = share * blockIdx.x, count = min(share, total - first);  // (count <= 0: nothing)
+  if (count > 0 && first >= upto - mine && first < upto) {
+    long long off = first - (upto - mine);
+    int s = s_lo;
+    for (long long n; off >= (n = blocks_of(s)); ++s) off -= n;
+    scan[10] = s, scan[11] = off;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  chain_release();
+  const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
+  TreeWalk walk;
+  walk.start(p, __shfl_sync(0xFFFFFFFFu, static_cast<int>(scan[10]), 0), __shfl_sync(0xFFFFFFFFu, scan[11], 0), count);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    bool ok = true;
+    int qc = 0;  // Q tiles loaded so far
+    int ks = 0, vs = 0;
+    uint32_t kph = 0, vph = 0;
+    const int boxes = TR_BLOCK / p.box_rows;
+    const uint32_t box_bytes = p.box_rows * 128;
+    // Lane l loads half l % 2 (64 columns) of box l / 2.
+    const int box = lane >> 1, half = lane & 1;
+    const bool loads = lane < 2 * boxes;
+    auto wait = [&](uint32_t b, uint32_t parity) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, TJX_ERR_WAIT_EMPTY)) != 0;
+    };
+    TreePortion u;
+    while (ok && walk.next(p, u)) {
+      const int32_t* table = p.page_indices + static_cast<size_t>(u.s) * p.pages_per_seq;
+      // Row of the cache (page * page_size + row) where this lane's box of block j starts. (An entry past the table or
+      // a page past the pool is clamped, as a gather's index is.)
+      auto cache_row = [&](int j) {
+        const int pos = j * TR_BLOCK + box * p.box_rows;
+        const int entry = pos / p.page_size;
+        const int page = table[min(entry, p.pages_per_seq - 1)];
+        return min(max(page, 0), p.num_pages - 1) * p.page_size + (pos - entry * p.page_size);
+      };
+      int next_row = loads ? cache_row(u.j0) : 0;
+      for (int r = 0; r < (u.two ? 2 : 1) && ok; ++r, ++qc) {
+        const int b = qc & 1;
+        ok = wait(q_empty(b), ((qc >> 1) & 1) ^ 1u);
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t dst = base + L::Q_OFF + b * L::Q_BYTES;
+          mbar_expect_tx(q_full(b), static_cast<uint32_t>(p.tile_nodes * p.group) * 256u);
+          const int tok = u.tok + r * p.tile_nodes;
+          tma_load_3d(dst, &map_q, 0, u.hk * p.group, tok, q_full(b));
+          tma_load_3d(dst + L::Q_BYTES / 2, &map_q, 64, u.hk * p.group, tok, q_full(b));
+        }
+        __syncwarp();
+      }
+      for (int j = u.j0; j < u.j1 && ok; ++j) {
+        const int row = next_row;
+        if (loads && j + 1 < u.j1) next_row = cache_row(j + 1);
+        ok = wait(k_empty(ks), kph ^ 1u);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(k_full(ks), L::KV_BYTES);
+        __syncwarp();
+        if (loads)
+          tma_load_3d(base + L::K_OFF + ks * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
+                      2 * u.hk, row, k_full(ks));
+        if (++ks == TR_K_STAGES) ks = 0, kph ^= 1u;
+        ok = wait(v_empty(vs), vph ^ 1u);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(v_full(vs), L::KV_BYTES);
+        __syncwarp();
+        if (loads)
+          tma_load_3d(base + L::V_OFF + vs * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
+                      2 * u.hk + 1, row, v_full(vs));
+        if (++vs == TR_V_STAGES) vs = 0, vph ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (whole warp; one lane issues)
+    const uint32_t idesc_qk = idesc_bf16_f32(128, TR_BLOCK, 0, 0);  // Q and K both K-major
+    const uint32_t idesc_pv = idesc_bf16_f32(128, TR_D, 0, 1);      // P from TMEM, V MN-major
+    auto wait = [&](uint32_t b, uint32_t parity, int code) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, code)) != 0;
+    };
+    TreeWalk ahead = walk;  // the scores' walk runs ahead of the outputs'
+    TreePortion a{}, b{};
+    int an = 0, bn = 0, a_jobs = 0, b_jobs = 0;  // job of the portion, its jobs
+    int ja = 0, jb = 0;                          // jobs issued so far
+    int ks = 0, vs = 0, qc = 0;
+    uint32_t kph = 0, vph = 0;
+    bool ok = true, more = true;
+    while (ok) {
+      if (more && an == a_jobs) {
+        more = ahead.next(p, a);
+        an = 0, a_jobs = more ? a.jobs : 0;
+      }
+      if (more) {
+        // Q K^T of job an: row tile an % 2 of block an / 2, or the one tile of block an.
+        const int r = a.two ? an & 1 : 0, qb = (qc + r) & 1;
+        if (an == r) ok = wait(q_full(qb), ((qc + r) >> 1) & 1, TJX_ERR_WAIT_FULL);
+        if (ok && r == 0) ok = wait(k_full(ks), kph, TJX_ERR_WAIT_FULL);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int t = ja & 1, sb = (ja >> 1) & 1;
+        const uint64_t q0 = smem_desc_sw128(base + L::Q_OFF + qb * L::Q_BYTES, 16, 1024);
+        const uint64_t k0 = smem_desc_sw128(base + L::K_OFF + ks * L::KV_BYTES, 16, 1024);
+        uint64_t qd[8], kd[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] *= alpha;
-    for (int i = 0; i < 32; ++i) {
-      const float w = __shfl_sync(0xFFFFFFFFu, e, i);
-      const long long r = __shfl_sync(0xFFFFFFFFu, row, i);
-      if (!((seen >> i) & 1)) continue;
-      const uint2 v = reinterpret_cast<const uint2*>(p.kv_cache + r + TR_D)[lane];
-      o[0] += w * bf16_lo(v.x), o[1] += w * bf16_hi(v.x), o[2] += w * bf16_lo(v.y), o[3] += w * bf16_hi(v.y);
+        for (int kk = 0; kk < 8; ++kk) {
+          qd[kk] = q0 + (((kk >> 2) * (L::Q_BYTES / 2) + (kk & 3) * 32) >> 4);
+          kd[kk] = k0 + (((kk >> 2) * (L::KV_BYTES / 2) + (kk & 3) * 32) >> 4);
+        }
+        mma_ss_x8_commit(tmem_base + t * 128 + sb * 64, qd, kd, idesc_qk, 0u, s_full(t, sb));
+        if (!a.two || r == 1) {
+          mma_commit_elected(k_empty(ks));
+          if (++ks == TR_K_STAGES) ks = 0, kph ^= 1u;
+        }
+        ++ja, ++an;
+        if (an + (a.two ? 1 - r : 0) == a_jobs) mma_commit_elected(q_empty(qb));  // the tile's last use
+        if (an == a_jobs) qc += a.two ? 2 : 1;
+      }
+      if (ja - jb > 2 || !more) {
+        if (jb == ja) break;
+        if (bn == b_jobs) {
+          walk.next(p, b);
+          bn = 0, b_jobs = b.jobs;
+        }
+        const int t = jb & 1, sb = (jb >> 1) & 1, r = b.two ? bn & 1 : 0;
+        if (r == 0) ok = wait(v_full(vs), vph, TJX_ERR_WAIT_FULL);
+        if (ok) ok = wait(p_ready(t, sb), (jb >> 2) & 1, TJX_ERR_WAIT_OTHER);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint64_t v0 = smem_desc_sw128(base + L::V_OFF + vs * L::KV_BYTES, L::KV_BYTES / 2, 1024);
+        uint64_t vd[4];
+        uint32_t pa[4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          vd[kk] = v0 + ((kk * 16 * 128) >> 4);
+          pa[kk] = tmem_base + t * 128 + sb * 64 + kk * 8;
+        }
+        mma_ts_x4_commit(tmem_base + 256 + t * 128, pa, vd, idesc_pv, bn >= 2 ? 1u : 0u, o_done(t, sb));
+        if (!b.two || r == 1) {
+          mma_commit_elected(v_empty(vs));
+          if (++vs == TR_V_STAGES) vs = 0, vph ^= 1u;
+        }
+        ++jb, ++bn;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax and output
+    const int t = (warp - 2) >> 2;  // group
+    const int quarter = warp & 3;   // TMEM lanes of this warp
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const int row = quarter * 32 + lane;  // of the tile
+    int jobs = 0, blocks = 0;    // of the portions before
+    int looked = 0, looked_both = 0, joined = 0;
+    bool ok = true;
+    auto wait = [&](uint32_t b, uint32_t parity, int code) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, code)) != 0;
+    };
+    // The product of the group's job c is in the output. A wait tells a barrier's phase from the one before it only, and
+    // the scores of job c say that job c - 2 is through, not job c - 1: so even and odd jobs have barriers of their own.
+    auto output_done = [&](int c) { return wait(o_done(t, c & 1), (c >> 1) & 1, TJX_ERR_WAIT_OTHER); };
+    if (threadIdx.x == 64) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    TreePortion u;
+    while (ok && walk.next(p, u)) {
+      const int n0 = (t - jobs) & 1;  // this group's first job of the portion
+      const int tile = u.two ? n0 : 0;
+      const int tile_nodes = u.two ? (tile == 0 ? p.tile_nodes : u.nodes - p.tile_nodes) : u.nodes;
+      const int rows = tile_nodes * p.group;
+      const bool active = quarter * 32 < rows;  // some row of this warp's is one
+      const int node = row / p.group;           // in its tile
+      const bool mine_valid = row < rows;
+      const int tok = u.tok + tile * p.tile_nodes + node;
+      const int32_t* mask = p.tree_mask + static_cast<size_t>(mine_valid ? tok : 0) * p.words;
+      const int words = mine_valid ? p.words : 0;
+      float m_used = TR_NOTHING, l = 0.f;
+      int last_job = -1;
+      for (int n = n0; n < u.jobs && ok; n += 2) {
+        const int c = (jobs + n) >> 1, sb = c & 1;  // the group's job
+        const int block = u.two ? n >> 1 : n, kv0 = (u.j0 + block) * TR_BLOCK;
+        const uint32_t s_tmem = tmem_base + lane_addr + t * 128 + sb * 64;
+        const uint32_t o_tmem = tmem_base + lane_addr + 256 + t * 128;
+        const bool special = kv0 + TR_BLOCK > min(u.ctx, u.end);  // positions some row does not see, or that are none
+        uint32_t bad[4] = {0, 0, 0, 0};
+        const int stage = (blocks + block) % TR_V_STAGES;
+        if (special) {
+          // What a row does not see must not reach it: zero times NaN is NaN. Rows of V past the end are zeroed, and
+          // rows holding anything but finite numbers too, which are then added by hand to the rows that see them.
+          ok = wait(v_full(stage), ((blocks + block) / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
+          if (!ok) break;
+          const int g_row = row >> 1, limit = u.end - kv0;
+          uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
+                                                g_row * 128);
+          bool odd = false;
+          if (g_row < limit) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint4 x = src[i];
+              odd |= not_finite_bf16x2(x.x) || not_finite_bf16x2(x.y) || not_finite_bf16x2(x.z) || not_finite_bf16x2(x.w);
+            }
+          }
+          uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
+          votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
+          volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
+          if (lane == 0) {
+            flags[quarter] = votes;
+            mbar_arrive(u.two ? v_seen_both : v_seen(t));
+          }
+          ok = u.two ? wait(v_seen_both, looked_both & 1, TJX_ERR_WAIT_OTHER) : wait(v_seen(t), looked & 1, TJX_ERR_WAIT_OTHER);
+          if (u.two) ++looked_both; else ++looked;
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bad[i] = flags[i];
+          if (g_row >= limit || ((flags[g_row >> 4] >> (2 * (g_row & 15))) & 1)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) src[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        ok = wait(s_full(t, sb), (c >> 1) & 1, TJX_ERR_WAIT_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t pk[32];
+        uint32_t see[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+        if (active) {
+          uint32_t v[2][32];
+          tmem_ld32(s_tmem, v[0]);
+          tmem_ld32(s_tmem + 32, v[1]);
+          if (special) {
+            see[0] = tree_bits(mask, words, kv0, u.ctx, u.end);
+            see[1] = tree_bits(mask, words, kv0 + 32, u.ctx, u.end);
+          }
+          tmem_wait_ld();
+          if (special) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((see[h] >> i) & 1)) v[h][i] = __float_as_uint(-INFINITY);
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[h][i]));
+          const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+          if (last_job < 0) {
+            m_used = fmaxf(m_blk, TR_NOTHING);
+          } else if (__any_sync(0xFFFFFFFFu, m_blk > m_used + TR_RESCALE)) {
+            const float m_new = fmaxf(m_used, m_blk), alpha = ex2(m_used - m_new);
+            m_used = m_new;
+            l *= alpha;
+            ok = output_done(c - 1);
+            if (!ok) break;
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[32];
+              tmem_ld32(o_tmem + i * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st32(o_tmem + i * 32, o);
+            }
+            tmem_wait_st();
+          }
+          // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention);
+          // the sum adds the unrounded values.
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float e0 = ex2(fmaf(__uint_as_float(v[h][i]), p.scale_log2e, -m_used));
+              const float e1 = ex2(fmaf(__uint_as_float(v[h][i + 1]), p.scale_log2e, -m_used));
+              sum[(i >> 1) & 1] += e0, sum[2 + ((i >> 1) & 1)] += e1;
+              pk[h * 16 + (i >> 1)] = pack_bf16(e0, e1);
+            }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st32(s_tmem, pk);
+          tmem_wait_st();
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(t, sb));
+        last_job = c;
+        if (active && (bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
+          // The rows of V that were taken out: added to the rows that see them, once this block's product is in.
+          ok = output_done(c);
+          if (!ok) break;
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int g = 0; g < TR_BLOCK; ++g) {
+            const uint32_t some = g < 32 ? (g < 16 ? bad[0] : bad[1]) : (g < 48 ? bad[2] : bad[3]);
+            if (!((some >> (2 * (g & 15))) & 1)) continue;
+            const bool sees = ((g < 32 ? see[0] : see[1]) >> (g & 31)) & 1;
+            uint32_t pair = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == g >> 1) pair = pk[i];
+            const float weight = (g & 1) ? bf16_hi(pair) : bf16_lo(pair);
+            const int pos = kv0 + g;  // (below the end)
+            const int page = min(max(p.page_indices[static_cast<size_t>(u.s) * p.pages_per_seq + pos / p.page_size], 0), p.num_pages - 1);
+            const uint32_t* vrow = reinterpret_cast<const uint32_t*>(
+                p.kv_cache + (((static_cast<size_t>(page) * p.page_size + pos % p.page_size) * p.Hkv + u.hk) * 2 + 1) * TR_D);
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[32];
+              tmem_ld32(o_tmem + i * 32, o);
+              tmem_wait_ld();
+              if (sees) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                  const uint32_t w = vrow[i * 16 + x];
+                  o[2 * x] = __float_as_uint(fmaf(weight, bf16_lo(w), __uint_as_float(o[2 * x])));
+                  o[2 * x + 1] = __float_as_uint(fmaf(weight, bf16_hi(w), __uint_as_float(o[2 * x + 1])));
+                }
+              }
+              tmem_st32(o_tmem + i * 32, o);
+              tmem_wait_st();
+            }
+          }
+          tc_fence_before_sync();
+        }
+      }
+      if (!ok) break;
+      // The portion's end: normalised rows, or a partial result for the join.
+      if (last_job >= 0) ok = output_done(last_job);
+      if (!ok) break;
+      const int part = 2 * blockIdx.x + (u.starts ? 1 : 0);
+      const int head = u.hk * p.group + row - node * p.group;
+      const size_t out_row = static_cast<size_t>(tok) * p.H + head;
+      const size_t part_row = static_cast<size_t>(part) * p.part_rows + tile * p.tile_nodes * p.group + row;
+      auto store32 = [&](int col, const float (&o)[32]) {  // 32 columns of this thread's row
+        if (u.whole) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * TR_D + col);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            dst[x] = make_uint4(pack_bf16(o[8 * x], o[8 * x + 1]), pack_bf16(o[8 * x + 2], o[8 * x + 3]),
+                                pack_bf16(o[8 * x + 4], o[8 * x + 5]), pack_bf16(o[8 * x + 6], o[8 * x + 7]));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + part_row * TR_D + col);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) dst[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+      };
+      if (u.two) {
+        tc_fence_after_sync();
+        const float inv = u.whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+        if (active) {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tmem_ld32(tmem_base + lane_addr + 256 + t * 128 + i * 32, o);
+            tmem_wait_ld();
+            float f[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) f[x] = __uint_as_float(o[x]) * inv;
+            if (mine_valid) store32(i * 32, f);
+          }
+          if (mine_valid && !u.whole) p.part_ml[part_row] = make_float2(m_used, l);
+        }
+        tc_fence_before_sync();
+      } else {
+        // Both groups have a part of the tile's blocks: they exchange their rows' maxima and sums and each joins one
+        // half of the columns.
+        stats[t * TR_ROWS + row] = make_float2(m_used, l);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(stats_ready);
+        ok = wait(stats_ready, joined & 1, TJX_ERR_WAIT_OTHER);
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (active) {
+          const float2 a = stats[row], b = stats[TR_ROWS + row];
+          const bool has[2] = {u.jobs > ((0 - jobs) & 1), u.jobs > ((1 - jobs) & 1)};  // the group had a job
+          const float m = fmaxf(a.x, b.x);
+          float w0 = ex2(a.x - m), w1 = ex2(b.x - m);
+          const float sum = a.y * w0 + b.y * w1;
+          if (u.whole) {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            w0 *= inv, w1 *= inv;
+          }
+#pragma unroll 1
+          for (int i = 2 * t; i < 2 * t + 2; ++i) {
+            float f[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) f[x] = 0.f;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (!has[g]) continue;
+              uint32_t o[32];
+              tmem_ld32(tmem_base + lane_addr + 256 + g * 128 + i * 32, o);
+              tmem_wait_ld();
+              const float w = g == 0 ? w0 : w1;
+#pragma unroll
+              for (int x = 0; x < 32; ++x) f[x] = fmaf(__uint_as_float(o[x]), w, f[x]);
+            }
+            if (mine_valid) store32(i * 32, f);
+          }
+          if (mine_valid && !u.whole && t == 0) p.part_ml[part_row] = make_float2(m, sum);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(outputs_read);
+        ok = wait(outputs_read, joined & 1, TJX_ERR_WAIT_OTHER);  // the outputs and the statistics may be overwritten
+        ++joined;
+        tc_fence_after_sync();
+      }
+      if (u.starts && !u.whole && threadIdx.x == 64)
+        p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + (u.after + share - 1) / share));
+      jobs += u.jobs, blocks += u.j1 - u.j0;
     }
   }
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;  // a row that sees nothing is zero
-  *dst = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort_flag) __nanosleep(100000);
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+constexpr int TJ_WARPS = 8;  // rows of a CTA
+
+// The units that several CTAs shared: a warp per row joins its partial results in the order of the blocks. And the rows
+// that no unit has, which stay the query.
+__global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
+  chain_wait();
+  const int lane = threadIdx.x & 31, x = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
+  const int4 join = p.joins[blockIdx.x];
+  if (x < join.y * p.group) {
+    const int first = blockIdx.x, n = join.w - first + 1;  // parts: 2 first + 1, 2 (first + 1), 2 (first + 2), ...
+    auto part_row = [&](int i) {
+      return static_cast<size_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.part_rows + x;
+    };
+    float m = TR_NOTHING;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[part_row(i)].x);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    float sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float w = 0.f;
+      if (i0 + lane < n) {
+        const float2 ml = p.part_ml[part_row(i0 + lane)];
+        w = ex2(ml.x - m);
+        sum += w * ml.y;
+      }
+      const int some = min(n - i0, 32);
+#pragma unroll 4
+      for (int i = 0; i < some; ++i) {
+        const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
+        const float4 v = reinterpret_cast<const float4*>(p.part_o + part_row(i0 + i) * TR_D)[lane];
+        o.x = fmaf(v.x, wi, o.x), o.y = fmaf(v.y, wi, o.y), o.z = fmaf(v.z, wi, o.z), o.w = fmaf(v.w, wi, o.w);
+      }
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const size_t row = static_cast<size_t>(join.x + x / p.group) * p.H + join.z * p.group + x % p.group;
+    reinterpret_cast<uint2*>(p.out + row * TR_D)[lane] =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  }
+  if (p.out != p.q) {
+    const int seqs = min(max(p.distribution[0], 0), p.S);
+    const int lo = min(max(p.cu_q_lens[0], 0), p.T), hi = min(max(p.cu_q_lens[seqs], lo), p.T);
+    const size_t units = static_cast<size_t>(p.H) * TR_D / 8;  // 16 bytes each
+    const size_t rest = (static_cast<size_t>(lo) + (p.T - hi)) * units;
+    const size_t step = static_cast<size_t>(gridDim.x) * gridDim.y * TJ_WARPS * 32;
+    for (size_t i = (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * TJ_WARPS * 32 + threadIdx.x; i < rest; i += step) {
+      const size_t at = i < lo * units ? i : i + static_cast<size_t>(hi - lo) * units;
+      reinterpret_cast<uint4*>(p.out)[at] = reinterpret_cast<const uint4*>(p.q)[at];
+    }
+  }
+}
+
+static size_t tree_align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+static int tree_part_rows(int T, int group) {
+  return static_cast<int>(std::min<long long>(2 * TR_ROWS, static_cast<long long>(T) * group));
 }
 
 }  // namespace tjx
 
 extern "C" size_t tjx_rpa_tree_attention_workspace_bytes(int T, int S, int H, int Hkv) {
-  if (T <= 0 || S <= 0 || H <= 0 || Hkv <= 0) return 0;
-  return 256;
+  using namespace tjx;
+  if (T <= 0 || S <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0) return 0;
+  const size_t ctas = check_device() == 0 ? sm_count() : 148;
+  const size_t rows = 2 * ctas * tree_part_rows(T, H / Hkv);
+  return tree_align256(ctas * sizeof(int4)) + tree_align256(rows * sizeof(float2)) + tree_align256(rows * TR_D * sizeof(float));
 }
 
 extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void* kv_cache, const int32_t* kv_lens,
@@ -123,11 +742,12 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
     return fail(TJX_E_ARG, "sizes must be positive");
   if (D != TR_D) return fail(TJX_E_ARG, "head dimension must be 128");
   if (H % Hkv != 0) return fail(TJX_E_ARG, "the query heads must be a multiple of the KV heads");
-  if (H / Hkv > 128) return fail(TJX_E_LIMIT, "at most 128 query heads per KV head");
+  if (H / Hkv > TR_ROWS) return fail(TJX_E_LIMIT, "at most 128 query heads per KV head");
   if (page_size <= 0 || page_size % 16 != 0) return fail(TJX_E_ARG, "page_size must be a multiple of 16");
   if (!(sm_scale > 0.f) || sm_scale > 1e30f) return fail(TJX_E_ARG, "sm_scale must be positive");
   if (static_cast<long long>(num_pages) * page_size >= (1ll << 31) || static_cast<long long>(T) * H >= (1ll << 31) ||
-      static_cast<long long>(S) * pages_per_seq >= (1ll << 31) || static_cast<long long>(pages_per_seq) * page_size >= (1ll << 31))
+      static_cast<long long>(S) * pages_per_seq >= (1ll << 31) ||
+      static_cast<long long>(pages_per_seq) * page_size >= (1ll << 31) - TR_BLOCK)
     return fail(TJX_E_LIMIT, "num_pages * page_size, pages_per_seq * page_size, S * pages_per_seq and T * H must fit in int32");
   for (const void* ptr : {q, static_cast<const void*>(out), kv_cache})
     if (reinterpret_cast<uintptr_t>(ptr) & 15u) return fail(TJX_E_ARG, "q, out and kv_cache must be 16-byte aligned");
@@ -142,8 +762,42 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
   p.distribution = distribution;
   p.T = T, p.S = S, p.H = H, p.Hkv = Hkv, p.group = H / Hkv, p.page_size = page_size, p.pages_per_seq = pages_per_seq;
   p.num_pages = num_pages, p.words = words, p.scale_log2e = sm_scale * TR_LOG2E;
-  const long long warps = static_cast<long long>(T) * H;
-  tree_simple_kernel<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.tile_nodes = TR_ROWS / p.group;
+  p.box_rows = std::min(page_size & -page_size, TR_BLOCK);
+  p.status = device_status_word();
+  if (p.status == nullptr) return fail(TJX_E_CUDA, "could not locate the device status word");
+  const int ctas = sm_count();
+  p.part_rows = tree_part_rows(T, p.group);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  p.joins = reinterpret_cast<int4*>(w), w += tree_align256(ctas * sizeof(int4));
+  p.part_ml = reinterpret_cast<float2*>(w), w += tree_align256(2ull * ctas * p.part_rows * sizeof(float2));
+  p.part_o = reinterpret_cast<float*>(w);
+
+  CUtensorMap mq, mkv;
+  {
+    const uint64_t dims[3] = {TR_D, static_cast<uint64_t>(H), static_cast<uint64_t>(T)};
+    const uint64_t strides[2] = {TR_D * 2, static_cast<uint64_t>(H) * TR_D * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.tile_nodes)};
+    if (int rc = make_tensor_map(&mq, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
+  {
+    const uint64_t dims[3] = {TR_D, static_cast<uint64_t>(Hkv) * 2, static_cast<uint64_t>(num_pages) * page_size};
+    const uint64_t strides[2] = {TR_D * 2, static_cast<uint64_t>(Hkv) * 2 * TR_D * 2};
+    const uint32_t box[3] = {64, 1, static_cast<uint32_t>(p.box_rows)};
+    if (int rc = make_tensor_map(&mkv, kv_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
+  static bool configured[64] = {};
+  int dev = 0;
+  TJX_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    TJX_CUDA(cudaFuncSetAttribute(tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeSmem::TOTAL));
+    configured[dev & 63] = true;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  tree_kernel<<<ctas, TR_THREADS, TreeSmem::TOTAL, s>>>(mq, mkv, p);
   TJX_CUDA(cudaGetLastError());
+  TJX_CUDA(launch_chained(tree_join_kernel, dim3(ctas, (p.part_rows + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, s, p));
   return 0;
 }
