@@ -28,15 +28,29 @@ def _stream() -> ctypes.c_void_p:
 
 
 def _need_cuda(*tensors: torch.Tensor) -> torch.device:
-    device = tensors[0].device
+    index = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("tilejax_b200 operators take CUDA tensors (there is no CPU path)")
-        if t.device != device:
+        if index < 0 or t.get_device() != index:
+            if not t.is_cuda or index < 0:
+                raise ValueError("tilejax_b200 operators take CUDA tensors (there is no CPU path)")
             raise ValueError("all tensors must be on the same device")
         if not t.is_contiguous():
             raise ValueError("tensors must be contiguous (row-major)")
-    return device
+    return tensors[0].device
+
+
+def _launch(device: torch.device, entry: str, *args) -> None:
+    """A call into the library on `device`'s current stream: pointers as integers (None: null), the stream appended. The
+    current device is changed only if it is another one: a few microseconds that a small operator is not worth."""
+    index = device.index
+    call = getattr(library(), entry)
+    if torch._C._cuda_getDevice() == index:
+        code = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != 0:
+        check(code)
 
 
 _table_cache: dict[tuple, torch.Tensor] = {}
@@ -442,13 +456,14 @@ def mla_decode(q_c: torch.Tensor, q_r: torch.Tensor, c_kv: torch.Tensor, k_rope:
 
 
 def _rpa_sizes(kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor) -> tuple[int, ...]:
-    if kv_cache.dim() != 5 or kv_cache.shape[3] != 2 or kv_cache.dtype != torch.bfloat16:
+    shape = kv_cache.shape
+    if len(shape) != 5 or shape[3] != 2 or kv_cache.dtype is not torch.bfloat16:
         raise ValueError("the cache is (pages, page_size, Hkv, 2, D) bfloat16: each head's key and value side by side")
-    num_pages, page_size, Hkv, _, D = kv_cache.shape
+    num_pages, page_size, Hkv, _, D = shape
     S = kv_lens.shape[0]
     if page_indices.dim() != 1 or S == 0 or page_indices.shape[0] % S:
         raise ValueError("page_indices is (S * pages_per_seq,), sequence s's pages at s * pages_per_seq")
-    if any(t.dtype != torch.int32 for t in (kv_lens, page_indices)):
+    if kv_lens.dtype is not torch.int32 or page_indices.dtype is not torch.int32:
         raise ValueError("kv_lens and page_indices must be int32")
     return num_pages, page_size, Hkv, D, S, page_indices.shape[0] // S
 
@@ -635,21 +650,17 @@ def ragged_paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
 # ------------------------------------------------------------------------------------------ a step over drafted tokens
 
 
-def _int32_vectors(**tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.dim() != 1:
-            raise ValueError(f"{name} must be an int32 vector")
+def _end(t: torch.Tensor) -> int:
+    """The address behind the last element."""
+    at = 1
+    for n, step in zip(t.shape, t.stride()):
+        at += (n - 1) * step
+    return t.data_ptr() + at * t.element_size()
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory from the first to the last element of the one meets that of the other."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-
-    def end(t):
-        return t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < _end(b) and b.data_ptr() < _end(a)
 
 
 class RpaStep(NamedTuple):
@@ -673,93 +684,122 @@ def rpa_plan(ctx_lens: torch.Tensor, q_lens: torch.Tensor, page_indices: torch.T
     is empty. `depths` (tokens,) gives drafted tokens their depth in the tree: the token's position is then ctx_lens[s]
     plus its depth, while its slot stays that of its index. `out` is written instead of new tensors; it may not overlap
     the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into ctx_lens)."""
-    inputs = [t for t in (ctx_lens, q_lens, page_indices, free_pages, n_free, pages_held, depths) if t is not None]
-    _int32_vectors(ctx_lens=ctx_lens, q_lens=q_lens, page_indices=page_indices, free_pages=free_pages, n_free=n_free)
-    S, T = ctx_lens.shape[0], int(tokens)
-    if S == 0 or q_lens.shape[0] != S or page_indices.shape[0] == 0 or page_indices.shape[0] % S:
+    inputs = [ctx_lens, q_lens, page_indices, free_pages, n_free]
+    for name, t in zip(("ctx_lens", "q_lens", "page_indices", "free_pages", "n_free"), inputs):
+        if t.dtype is not torch.int32 or t.dim() != 1:
+            raise ValueError(f"{name} must be an int32 vector")
+    S, T, entries = ctx_lens.shape[0], int(tokens), page_indices.shape[0]
+    if S == 0 or q_lens.shape[0] != S or entries == 0 or entries % S:
         raise ValueError("ctx_lens and q_lens are (S,), page_indices (S * pages_per_seq,)")
     if n_free.shape[0] < 1:
         raise ValueError("n_free holds the number of free pages")
-    if pages_held is not None and (pages_held.shape != (S,) or pages_held.dtype != torch.int32):
-        raise ValueError("pages_held is int32 (S,)")
-    if depths is not None and (depths.shape != (T,) or depths.dtype != torch.int32):
-        raise ValueError("depths is int32 (tokens,)")
+    if pages_held is not None:
+        inputs.append(pages_held)
+        if pages_held.shape != (S,) or pages_held.dtype is not torch.int32:
+            raise ValueError("pages_held is int32 (S,)")
+    if depths is not None:
+        inputs.append(depths)
+        if depths.shape != (T,) or depths.dtype is not torch.int32:
+            raise ValueError("depths is int32 (tokens,)")
     if T < 0 or page_size <= 0:
         raise ValueError("page_size must be positive and tokens not negative")
     device = _need_cuda(*inputs)
     if out is None:
-        out = RpaStep(*torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device).split([S, S + 1, T, T, S, 2]))
+        out = RpaStep(*torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device)
+                      .split_with_sizes((S, S + 1, T, T, S, 2)))
     else:
         _need_cuda(ctx_lens, *out)
-        if [tuple(t.shape) for t in out] != [(S,), (S + 1,), (T,), (T,), (S,), (2,)] or any(t.dtype != torch.int32 for t in out):
+        if [tuple(t.shape) for t in out] != [(S,), (S + 1,), (T,), (T,), (S,), (2,)] or any(t.dtype is not torch.int32 for t in out):
             raise ValueError("out is a step of other sizes")
         if any(_overlap(a, b) for a in out for b in inputs):
             raise ValueError("out overlaps an input")
-    with torch.cuda.device(device):
-        check(library().tjx_rpa_plan(_ptr(ctx_lens), _ptr(q_lens), _ptr(pages_held), _ptr(depths), _ptr(page_indices),
-                                     _ptr(free_pages), _ptr(n_free), free_pages.shape[0], S, T,
-                                     page_indices.shape[0] // S, page_size, *map(_ptr, out), _stream()))
+    _launch(device, "tjx_rpa_plan", ctx_lens.data_ptr(), q_lens.data_ptr(), None if pages_held is None else pages_held.data_ptr(),
+            None if depths is None else depths.data_ptr(), page_indices.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(),
+            free_pages.shape[0], S, T, entries // S, page_size, *[t.data_ptr() for t in out])
     return out
 
 
-def _heads(name: str, t: torch.Tensor, tokens: int, heads: int | None, D: int) -> None:
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[0] != tokens or t.shape[2] != D or \
-            (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be bfloat16 ({tokens}, {'heads' if heads is None else heads}, {D})")
-    if t.stride(2) != 1 or t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
+_NormRopeStrides = ctypes.c_int64 * 10
+
+
+def _heads(name: str, t: torch.Tensor, tokens: int, D: int) -> tuple[int, int, int]:
+    """Heads, token stride and head stride of a (tokens, heads, D) operand."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not torch.bfloat16 or shape[0] != tokens or shape[2] != D:
+        raise ValueError(f"{name} must be bfloat16 ({tokens}, heads, {D})")
+    token, head, dense = t.stride()
+    if dense != 1 or token % 4 or head % 4 or t.data_ptr() % 8:
         raise ValueError(f"{name}'s last dimension must be dense, its strides multiples of 4 elements, its data 8-byte aligned")
+    return shape[1], token, head
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a is b or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride())
 
 
 def _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, kv_cache, slots, eps, interleaved):
     if q.dim() != 3:
         raise ValueError("q is (T, H, D)")
     T, H, D = q.shape
-    Hkv = k.shape[1] if k.dim() == 3 else 0
-    _heads("q", q, T, None, D)
-    _heads("k", k, T, None, D)
+    _, q_tok, q_head = _heads("q", q, T, D)
+    Hkv, k_tok, k_head = _heads("k", k, T, D)
     if (q_gamma is None) != (k_gamma is None):
         raise ValueError("q_gamma and k_gamma are given together or not at all")
-    for g in (q_gamma, k_gamma):
-        if g is not None and (g.shape != (D,) or g.dtype != torch.bfloat16 or not g.is_contiguous() or g.data_ptr() % 8):
-            raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
-    if positions.shape != (T,) or positions.dtype != torch.int32:
+    dense = [positions, cos_sin]
+    if q_gamma is not None:
+        dense += (q_gamma, k_gamma)
+        for g in (q_gamma, k_gamma):
+            if g.shape != (D,) or g.dtype is not torch.bfloat16 or g.data_ptr() % 8:
+                raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
+    if positions.shape != (T,) or positions.dtype is not torch.int32:
         raise ValueError("positions is int32 (T,)")
-    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[1] > D or cos_sin.shape[1] % 8 \
+    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32 or cos_sin.shape[1] > D or cos_sin.shape[1] % 8 \
             or cos_sin.shape[0] == 0 or cos_sin.data_ptr() % 16:
         raise ValueError("cos_sin is float32 (max_positions, rot), rot a multiple of 8 up to the head dimension, 16-byte aligned")
-    device = _need_cuda(positions, cos_sin, *(t for t in (q_gamma, k_gamma, slots) if t is not None))
-    used = [t for t in (q, k, v) if t is not None]
-    if any(t.device != device for t in used):
-        raise ValueError("all tensors must be on the same device")
+    used = (q, k)
+    v_tok = v_head = slots_ptr = n_slots = 0
+    if kv_cache is not None:
+        used = (q, k, v)
+        _, v_tok, v_head = _heads("v", v, T, D)
+        dense += (slots, kv_cache)
+        slots_ptr, n_slots = slots.data_ptr(), kv_cache.shape[0] * kv_cache.shape[1]
+    device = _need_cuda(*dense)
+    for t in used:
+        if t.get_device() != device.index:
+            raise ValueError("all tensors must be on the same device")
     if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=q.dtype, device=device)
-    elif q_out is not q:
-        _heads("the queries' output", q_out, T, H, D)
-        if q_out.device != device or any(_overlap(q_out, t) for t in used if not _same(q_out, q)):
-            raise ValueError("the queries' output is q itself or memory of its own, on q's device")
+        q_out = torch.empty((T, H, D), dtype=torch.bfloat16, device=device)
+        qo_tok, qo_head = H * D, D
+    else:
+        heads, qo_tok, qo_head = _heads("the queries' output", q_out, T, D)
+        if heads != H or q_out.device != device or any(_overlap(q_out, t) for t in used if not _same(q_out, q)):
+            raise ValueError("the queries' output is q itself or memory of its own, like q")
+    ko_tok = ko_head = 0
     if kv_cache is None:
         if k_out is None:
-            k_out = torch.empty((T, Hkv, D), dtype=k.dtype, device=device)
-        elif k_out is not k:
-            _heads("the keys' output", k_out, T, Hkv, D)
-            if k_out.device != device or any(_overlap(k_out, t) for t in (*used, q_out) if not _same(k_out, k)):
-                raise ValueError("the keys' output is k itself or memory of its own, on k's device")
-    elif any(_overlap(kv_cache, t) for t in (*used, q_out)):
-        raise ValueError("the cache overlaps an operand")
+            k_out = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
+            ko_tok, ko_head = Hkv * D, D
+        else:
+            heads, ko_tok, ko_head = _heads("the keys' output", k_out, T, D)
+            if heads != Hkv or k_out.device != device \
+                    or any(_overlap(k_out, t) for t in (q, k, q_out) if not _same(k_out, k)):
+                raise ValueError("the keys' output is k itself or memory of its own, like k")
+    else:
+        lo = kv_cache.data_ptr()
+        hi = lo + 2 * kv_cache.numel()
+        for at, heads, token, head in ((q.data_ptr(), H, q_tok, q_head), (k.data_ptr(), Hkv, k_tok, k_head),
+                                       (v.data_ptr(), Hkv, v_tok, v_head), (q_out.data_ptr(), H, qo_tok, qo_head)):
+            if at < hi and at + 2 * ((T - 1) * token + (heads - 1) * head + D) > lo:
+                raise ValueError("the cache overlaps an operand")
     if T == 0:
         return q_out, k_out
-    strides = (ctypes.c_int64 * 10)(*(x for t in (q, k, k if v is None else v, q_out, k if k_out is None else k_out)
-                                      for x in t.stride()[:2]))
-    with torch.cuda.device(device):
-        check(library().tjx_norm_rope_bf16(
-            _ptr(q), _ptr(k), _ptr(v), strides, _ptr(q_gamma), _ptr(k_gamma), _ptr(positions), _ptr(cos_sin), _ptr(slots),
-            _ptr(q_out), _ptr(k_out), _ptr(kv_cache), T, H, Hkv, D, cos_sin.shape[1], cos_sin.shape[0], int(interleaved),
-            0 if kv_cache is None else kv_cache.shape[0] * kv_cache.shape[1], float(eps), _stream()))
+    strides = _NormRopeStrides(q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head)
+    _launch(device, "tjx_norm_rope_bf16", q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), strides,
+            None if q_gamma is None else q_gamma.data_ptr(), None if k_gamma is None else k_gamma.data_ptr(),
+            positions.data_ptr(), cos_sin.data_ptr(), slots_ptr or None, q_out.data_ptr(),
+            None if k_out is None else k_out.data_ptr(), None if kv_cache is None else kv_cache.data_ptr(), T, H, Hkv, D,
+            cos_sin.shape[1], cos_sin.shape[0], 1 if interleaved else 0, n_slots, eps)
     return q_out, k_out
-
-
-def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None,
@@ -782,18 +822,21 @@ def rpa_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gam
     """`qk_norm_rope` with the cache write in the same pass: the turned key and the value of token t go to row slots[t]
     (page * page_size + row, as `rpa_plan` gives it; out of range: not written; no slot twice) of the cache
     (pages, page_size, Hkv, 2, D), IN PLACE. Returns (q', the cache); `out=q` updates the queries in place."""
-    if kv_cache.dim() != 5 or kv_cache.shape[3] != 2 or kv_cache.dtype != torch.bfloat16 or not kv_cache.is_contiguous() \
-            or kv_cache.numel() == 0:
+    if kv_cache.dim() != 5 or kv_cache.shape[3] != 2 or kv_cache.dtype is not torch.bfloat16 or kv_cache.numel() == 0:
         raise ValueError("the cache is (pages, page_size, Hkv, 2, D) bfloat16: each head's key and value side by side")
     if q.dim() != 3 or k.shape != v.shape or k.shape[1:] != (kv_cache.shape[2], kv_cache.shape[4]):
         raise ValueError("q is (T, H, D), k and v (T, Hkv, D) with the cache's Hkv and D")
     if kv_cache.shape[0] * kv_cache.shape[1] >= 1 << 31:
         raise ValueError("the cache's rows must fit in int32")
-    if slots.shape != (q.shape[0],) or slots.dtype != torch.int32 or slots.device != kv_cache.device:
-        raise ValueError("slots is int32 (T,), on the cache's device")
-    _heads("v", v, q.shape[0], k.shape[1], q.shape[2])
+    if slots.shape != (q.shape[0],) or slots.dtype is not torch.int32:
+        raise ValueError("slots is int32 (T,)")
     q_out, _ = _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, out, None, kv_cache, slots, eps, interleaved)
     return q_out, kv_cache
+
+
+@lru_cache(maxsize=256)
+def _tree_workspace_bytes(T: int, S: int, H: int, Hkv: int) -> int:
+    return int(library().tjx_rpa_tree_attention_workspace_bytes(T, S, H, Hkv))
 
 
 def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor,
@@ -806,13 +849,13 @@ def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.T
     the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
     the sequences from distribution[0] on. `out=q` updates in place."""
     num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
-    if q.dim() != 3 or q.shape[2] != D or q.dtype != torch.bfloat16:
+    if q.dim() != 3 or q.shape[2] != D or q.dtype is not torch.bfloat16:
         raise ValueError("q is (T, H, D) bfloat16")
     T, H, _ = q.shape
-    if cu_q_lens.shape != (S + 1,) or distribution.shape != (3,) or cu_q_lens.dtype != torch.int32 \
-            or distribution.dtype != torch.int32:
+    if cu_q_lens.shape != (S + 1,) or distribution.shape != (3,) or cu_q_lens.dtype is not torch.int32 \
+            or distribution.dtype is not torch.int32:
         raise ValueError("cu_q_lens is int32 (S + 1,), distribution int32 (3,)")
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.shape[1] == 0 or tree_mask.dtype != torch.int32:
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.shape[1] == 0 or tree_mask.dtype is not torch.int32:
         raise ValueError("tree_mask is int32 (T, words), 32 new tokens a word")
     device = _need_cuda(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution)
     if out is None:
@@ -823,14 +866,11 @@ def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.T
         raise ValueError("out is q itself or memory of its own")
     if T == 0:
         return out
-    with torch.cuda.device(device):
-        need = int(library().tjx_rpa_tree_attention_workspace_bytes(T, S, H, Hkv))
-        ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
-        ws_ptr = (ws.data_ptr() + 255) & ~255
-        check(library().tjx_rpa_tree_attention_bf16(
-            _ptr(q), _ptr(out), _ptr(kv_cache), _ptr(kv_lens), _ptr(page_indices), _ptr(cu_q_lens), _ptr(tree_mask),
-            _ptr(distribution), T, S, H, Hkv, D, tree_mask.shape[1], page_size, pps, num_pages, float(sm_scale),
-            ctypes.c_void_p(ws_ptr), need, _stream()))
+    need = _tree_workspace_bytes(T, S, H, Hkv)
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=device)  # (of the stream it is used on: no other may get it early)
+    _launch(device, "tjx_rpa_tree_attention_bf16", q.data_ptr(), out.data_ptr(), kv_cache.data_ptr(), kv_lens.data_ptr(),
+            page_indices.data_ptr(), cu_q_lens.data_ptr(), tree_mask.data_ptr(), distribution.data_ptr(), T, S, H, Hkv, D,
+            tree_mask.shape[1], page_size, pps, num_pages, sm_scale, (ws.data_ptr() + 255) & ~255, need)
     return out
 
 
@@ -842,22 +882,21 @@ def rpa_commit(kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torc
     its tokens. A path ends in front of an entry that does not ascend or is no new token. Returns the lengths, int32
     (S,), `out` if given (not kv_lens itself)."""
     num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
-    if cu_q_lens.shape != (S + 1,) or cu_q_lens.dtype != torch.int32:
+    if cu_q_lens.shape != (S + 1,) or cu_q_lens.dtype is not torch.int32:
         raise ValueError("cu_q_lens is int32 (S + 1,)")
-    if paths.dim() != 2 or paths.shape[0] != S or paths.shape[1] == 0 or paths.dtype != torch.int32 \
-            or n_accepted.shape != (S,) or n_accepted.dtype != torch.int32:
+    if paths.dim() != 2 or paths.shape[0] != S or paths.shape[1] == 0 or paths.dtype is not torch.int32 \
+            or n_accepted.shape != (S,) or n_accepted.dtype is not torch.int32:
         raise ValueError("paths is int32 (S, P), n_accepted int32 (S,)")
     device = _need_cuda(kv_cache, kv_lens, page_indices, cu_q_lens, paths, n_accepted)
     if out is None:
         out = torch.empty(S, dtype=torch.int32, device=device)
-    elif out.shape != (S,) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != device:
+    elif out.shape != (S,) or out.dtype is not torch.int32 or not out.is_contiguous() or out.device != device:
         raise ValueError("out is int32 (S,), on the cache's device")
     elif any(_overlap(out, t) for t in (kv_lens, page_indices, cu_q_lens, paths, n_accepted)):
         raise ValueError("out overlaps an input")
-    with torch.cuda.device(device):
-        check(library().tjx_rpa_commit_bf16(_ptr(kv_cache), _ptr(kv_lens), _ptr(page_indices), _ptr(cu_q_lens), _ptr(paths),
-                                            _ptr(n_accepted), _ptr(out), S, paths.shape[1], Hkv, D, page_size, pps,
-                                            num_pages, _stream()))
+    _launch(device, "tjx_rpa_commit_bf16", kv_cache.data_ptr(), kv_lens.data_ptr(), page_indices.data_ptr(),
+            cu_q_lens.data_ptr(), paths.data_ptr(), n_accepted.data_ptr(), out.data_ptr(), S, paths.shape[1], Hkv, D,
+            page_size, pps, num_pages)
     return out
 
 
