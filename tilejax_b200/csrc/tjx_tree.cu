@@ -14,13 +14,17 @@
 // (running maximum, sum, unnormalised rows) that tree_join_kernel joins in order. One persistent CTA per SM:
 //
 //   warp 0      producer: TMA loads of Q (a buffer per row tile), K and V blocks (boxes of at most a page) into rings
-//   warp 1      MMA issuer: S = Q K^T of two jobs ahead of O += P V, P read from TMEM
-//   warps 2-5   softmax of the even jobs, warps 6-9 of the odd ones (a thread owns a row)
+//   warps 1, 2  MMA issuers, one for each group: S = Q K^T one job ahead of O += P V, P read from TMEM
+//   warps 3-6   softmax of the one group, warps 7-10 of the other (a thread owns a row)
 //
-// A job is (row tile, block). With two row tiles the jobs of a block are its two tiles; with one tile they are
-// successive blocks, so the two softmax groups each keep a running maximum, sum and output over half of the blocks and
-// join them in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
+// A job is (row tile, block). With two row tiles each group (an issuer and its four softmax warps) has one of them; with
+// one tile the groups take the even and the odd blocks and each keep a running maximum, sum and output over theirs,
+// which they join in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
 // the scores), so that the next scores are made while it works, and 128 columns of output.
+//
+// A wait tells a barrier's phase from the one before it only. So whoever waits on a ring slot must have seen its use
+// before: rings have an even number of slots and blocks keep their parity over the whole run, so that a group finds
+// its blocks in the same slots always.
 #include <algorithm>
 
 #include "tjx_host.cuh"
@@ -34,8 +38,8 @@ constexpr int TR_D = 128;
 constexpr int TR_ROWS = 128;   // rows of a tile
 constexpr int TR_BLOCK = 64;   // positions of a block
 constexpr int TR_K_STAGES = 4;
-constexpr int TR_V_STAGES = 5;  // a V block is held longer: until its probabilities are made
-constexpr int TR_THREADS = 320;
+constexpr int TR_V_STAGES = 4;
+constexpr int TR_THREADS = 352;
 constexpr float TR_LOG2E = 1.4426950408889634f;
 constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a row that has seen nothing
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
@@ -65,10 +69,11 @@ struct TreeSmem {
   static constexpr int V_OFF = K_OFF + TR_K_STAGES * KV_BYTES;
   static constexpr int STAT_OFF = V_OFF + TR_V_STAGES * KV_BYTES;  // float2[2][128]: maximum and sum of each group's rows
   static constexpr int BAD_OFF = STAT_OFF + 2 * TR_ROWS * 8;       // uint32[2 groups][2][4]: rows of V that are not finite
-  static constexpr int SCAN_OFF = BAD_OFF + 64;                    // long long[10], and where this CTA starts
+  static constexpr int SCAN_OFF = BAD_OFF + 64;                    // long long[11], and where this CTA starts
   static constexpr int BAR_OFF = SCAN_OFF + 160;
   static constexpr int TOTAL = BAR_OFF + 512 + 1024;
 };
+static_assert(TR_K_STAGES % 2 == 0 && TR_V_STAGES % 2 == 0, "a slot's blocks are of one parity");
 static_assert(TreeSmem::TOTAL <= 232448, "shared memory of one CTA");
 
 // One sequence's sizes, clamped to what the arrays hold.
@@ -94,7 +99,6 @@ struct TreePortion {
   int node0;             // (first node's index in its sequence)
   int j0, j1;            // blocks of the unit
   bool whole, starts;    // all of the unit's blocks; its first block among them
-  int jobs;              // softmax jobs: blocks, twice as many with two row tiles
   bool two;              // two row tiles
   long long after;       // blocks of the unit behind this portion
 };
@@ -129,7 +133,6 @@ struct TreeWalk {
     o.j0 = j, o.j1 = j + take;
     o.starts = j == 0, o.whole = o.starts && o.j1 == q.blocks;
     o.after = q.blocks - o.j1;
-    o.jobs = o.two ? 2 * take : take;
     left -= take, j += take;
     if (j == q.blocks) {
       j = 0;
@@ -195,8 +198,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < N_BARS; ++i) {
-      // p_ready, v_seen: the warps of a group; the next three: of both
-      const int arrivals = (i >= 8 && i < 12) || i == 16 || i == 17 ? 4 : i >= 18 && i < RING ? 8 : 1;
+      // p_ready, v_seen: the warps of a group; the next three: of both. A Q, K or V buffer is free when both issuers say
+      // so (where only one uses it, the producer speaks for the other).
+      const bool by_both = i == 2 || i == 3 || (i >= RING + TR_K_STAGES && i < RING + 2 * TR_K_STAGES) ||
+                           i >= RING + 2 * TR_K_STAGES + TR_V_STAGES;
+      const int arrivals = (i >= 8 && i < 12) || i == 16 || i == 17 ? 4 : i >= 18 && i < RING ? 8 : by_both ? 2 : 1;
       mbar_init(bar + 8u * i, arrivals);
     }
     *abort_flag = 0;
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     long long off = first - (upto - mine);
     int s = s_lo;
     for (long long n; off >= (n = blocks_of(s)); ++s) off -= n;
-    scan[10] = s, scan[11] = off;
+    scan[11] = s, scan[12] = off;
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   chain_release();
   const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
   TreeWalk walk;
-  walk.start(p, __shfl_sync(0xFFFFFFFFu, static_cast<int>(scan[10]), 0), __shfl_sync(0xFFFFFFFFu, scan[11], 0), count);
+  walk.start(p, __shfl_sync(0xFFFFFFFFu, static_cast<int>(scan[11]), 0), __shfl_sync(0xFFFFFFFFu, scan[12], 0), count);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
@@ -285,6 +291,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           const int tok = u.tok + r * p.tile_nodes;
           tma_load_3d(dst, &map_q, 0, u.hk * p.group, tok, q_full(b));
           tma_load_3d(dst + L::Q_BYTES / 2, &map_q, 64, u.hk * p.group, tok, q_full(b));
+          if (u.two) mbar_arrive(q_empty(b));  // one issuer uses it
         }
         __syncwarp();
       }
@@ -298,6 +305,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (loads)
           tma_load_3d(base + L::K_OFF + ks * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
                       2 * u.hk, row, k_full(ks));
+        if (lane == 0 && !u.two) mbar_arrive(k_empty(ks));
         if (++ks == TR_K_STAGES) ks = 0, kph ^= 1u;
         ok = wait(v_empty(vs), vph ^ 1u);
         if (!ok) break;
@@ -306,63 +314,71 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (loads)
           tma_load_3d(base + L::V_OFF + vs * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
                       2 * u.hk + 1, row, v_full(vs));
+        if (lane == 0 && !u.two) mbar_arrive(v_empty(vs));
         if (++vs == TR_V_STAGES) vs = 0, vph ^= 1u;
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer (whole warp; one lane issues)
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ MMA issuers (whole warps; one lane issues)
+    // One issuer for both groups was the kernel's limit: some 1700 cycles a job, of which a tile's MMAs are 600 and the
+    // rest waits that find their barrier ready, descriptors and commits, one after the other.
+    const int t = warp - 1;
     const uint32_t idesc_qk = idesc_bf16_f32(128, TR_BLOCK, 0, 0);  // Q and K both K-major
     const uint32_t idesc_pv = idesc_bf16_f32(128, TR_D, 0, 1);      // P from TMEM, V MN-major
     auto wait = [&](uint32_t b, uint32_t parity, int code) {
       return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, code)) != 0;
     };
+    // A group's blocks of a portion: all of them, or with one row tile those of its parity, counted over the run.
+    auto first_of = [&](const TreePortion& u, int before) { return u.two ? 0 : (t - before) & 1; };
     TreeWalk ahead = walk;  // the scores' walk runs ahead of the outputs'
     TreePortion a{}, b{};
-    int an = 0, bn = 0, a_jobs = 0, b_jobs = 0;  // job of the portion, its jobs
-    int ja = 0, jb = 0;                          // jobs issued so far
-    int ks = 0, vs = 0, qc = 0;
-    uint32_t kph = 0, vph = 0;
+    int ia = 0, ib = 0;              // block of the portion
+    int a_blocks = 0, b_blocks = 0;  // blocks of the portions before
+    int ca = 0, cb = 0;              // jobs issued so far
+    int qc = 0;                      // Q tiles of the portions before
     bool ok = true, more = true;
     while (ok) {
-      if (more && an == a_jobs) {
+      while (ok && more && ia >= a.j1 - a.j0) {  // (a portion of one block has none for one of the groups)
+        a_blocks += a.j1 - a.j0, qc += a.nodes == 0 ? 0 : a.two ? 2 : 1;
         more = ahead.next(p, a);
-        an = 0, a_jobs = more ? a.jobs : 0;
+        if (!more) break;
+        ia = first_of(a, a_blocks);
+        for (int q = qc; q < qc + (a.two ? 2 : 1) && ok; ++q) ok = wait(q_full(q & 1), (q >> 1) & 1, TJX_ERR_WAIT_FULL);
+        if (ok && ia >= a.j1 - a.j0 && elect_one()) mbar_arrive(q_empty(qc & 1));
       }
+      if (!ok) break;
       if (more) {
-        // Q K^T of job an: row tile an % 2 of block an / 2, or the one tile of block an.
-        const int r = a.two ? an & 1 : 0, qb = (qc + r) & 1;
-        if (an == r) ok = wait(q_full(qb), ((qc + r) >> 1) & 1, TJX_ERR_WAIT_FULL);
-        if (ok && r == 0) ok = wait(k_full(ks), kph, TJX_ERR_WAIT_FULL);
+        // Q K^T
+        const int block = a_blocks + ia, q_buffer = (qc + (a.two ? t : 0)) & 1;
+        const int ks = block % TR_K_STAGES;
+        ok = wait(k_full(ks), (block / TR_K_STAGES) & 1, TJX_ERR_WAIT_FULL);
         if (!ok) break;
         tc_fence_after_sync();
-        const int t = ja & 1, sb = (ja >> 1) & 1;
-        const uint64_t q0 = smem_desc_sw128(base + L::Q_OFF + qb * L::Q_BYTES, 16, 1024);
-        const uint64_t k0 = smem_desc_sw128(base + L::K_OFF + ks * L::KV_BYTES, 16, 1024);
+        const uint32_t qa = base + L::Q_OFF + q_buffer * L::Q_BYTES, ka = base + L::K_OFF + ks * L::KV_BYTES;
+        const uint64_t q0 = smem_desc_sw128(qa, 16, 1024), k0 = smem_desc_sw128(ka, 16, 1024);
         uint64_t qd[8], kd[8];
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           qd[kk] = q0 + (((kk >> 2) * (L::Q_BYTES / 2) + (kk & 3) * 32) >> 4);
           kd[kk] = k0 + (((kk >> 2) * (L::KV_BYTES / 2) + (kk & 3) * 32) >> 4);
         }
-        mma_ss_x8_commit(tmem_base + t * 128 + sb * 64, qd, kd, idesc_qk, 0u, s_full(t, sb));
-        if (!a.two || r == 1) {
-          mma_commit_elected(k_empty(ks));
-          if (++ks == TR_K_STAGES) ks = 0, kph ^= 1u;
-        }
-        ++ja, ++an;
-        if (an + (a.two ? 1 - r : 0) == a_jobs) mma_commit_elected(q_empty(qb));  // the tile's last use
-        if (an == a_jobs) qc += a.two ? 2 : 1;
+        mma_ss_x8_commit(tmem_base + t * 128 + (ca & 1) * 64, qd, kd, idesc_qk, 0u, s_full(t, ca & 1));
+        mma_commit_elected(k_empty(ks));
+        ia += a.two ? 1 : 2, ++ca;
+        if (ia >= a.j1 - a.j0) mma_commit_elected(q_empty(q_buffer));  // this group's last use of the tile
       }
-      if (ja - jb > 2 || !more) {
-        if (jb == ja) break;
-        if (bn == b_jobs) {
+      if (ca - cb > 1 || !more) {
+        if (cb == ca) break;
+        while (ib >= b.j1 - b.j0) {
+          b_blocks += b.j1 - b.j0;
           walk.next(p, b);
-          bn = 0, b_jobs = b.jobs;
+          ib = first_of(b, b_blocks);
         }
-        const int t = jb & 1, sb = (jb >> 1) & 1, r = b.two ? bn & 1 : 0;
-        if (r == 0) ok = wait(v_full(vs), vph, TJX_ERR_WAIT_FULL);
-        if (ok) ok = wait(p_ready(t, sb), (jb >> 2) & 1, TJX_ERR_WAIT_OTHER);
+        // P V
+        const int block = b_blocks + ib, vs = block % TR_V_STAGES, sb = cb & 1;
+        ok = wait(v_full(vs), (block / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
+        if (ok) ok = wait(p_ready(t, sb), (cb >> 1) & 1, TJX_ERR_WAIT_OTHER);
         if (!ok) break;
         tc_fence_after_sync();
         const uint64_t v0 = smem_desc_sw128(base + L::V_OFF + vs * L::KV_BYTES, L::KV_BYTES / 2, 1024);
@@ -373,22 +389,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           vd[kk] = v0 + ((kk * 16 * 128) >> 4);
           pa[kk] = tmem_base + t * 128 + sb * 64 + kk * 8;
         }
-        mma_ts_x4_commit(tmem_base + 256 + t * 128, pa, vd, idesc_pv, bn >= 2 ? 1u : 0u, o_done(t, sb));
-        if (!b.two || r == 1) {
-          mma_commit_elected(v_empty(vs));
-          if (++vs == TR_V_STAGES) vs = 0, vph ^= 1u;
-        }
-        ++jb, ++bn;
+        mma_ts_x4_commit(tmem_base + 256 + t * 128, pa, vd, idesc_pv, ib == first_of(b, b_blocks) ? 0u : 1u, o_done(t, sb));
+        mma_commit_elected(v_empty(vs));
+        ib += b.two ? 1 : 2, ++cb;
       }
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax and output
-    const int t = (warp - 2) >> 2;  // group
+    const int t = (warp - 3) >> 2;  // group
     const int quarter = warp & 3;   // TMEM lanes of this warp
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;  // of the tile
-    int jobs = 0, blocks = 0;    // of the portions before
+    int c = 0, blocks = 0;  // jobs of this group, and blocks of the portions before
     int looked = 0, looked_both = 0, joined = 0;
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t parity, int code) {
@@ -397,11 +410,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     // The product of the group's job c is in the output. A wait tells a barrier's phase from the one before it only, and
     // the scores of job c say that job c - 2 is through, not job c - 1: so even and odd jobs have barriers of their own.
     auto output_done = [&](int c) { return wait(o_done(t, c & 1), (c >> 1) & 1, TJX_ERR_WAIT_OTHER); };
-    if (threadIdx.x == 64) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 96) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     TreePortion u;
     while (ok && walk.next(p, u)) {
-      const int n0 = (t - jobs) & 1;  // this group's first job of the portion
-      const int tile = u.two ? n0 : 0;
+      const int n_blocks = u.j1 - u.j0;
+      const int tile = u.two ? t : 0;
       const int tile_nodes = u.two ? (tile == 0 ? p.tile_nodes : u.nodes - p.tile_nodes) : u.nodes;
       const int rows = tile_nodes * p.group;
       const bool active = quarter * 32 < rows;  // some row of this warp's is one
@@ -412,9 +425,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       const int words = mine_valid ? p.words : 0;
       float m_used = TR_NOTHING, l = 0.f;
       int last_job = -1;
-      for (int n = n0; n < u.jobs && ok; n += 2) {
-        const int c = (jobs + n) >> 1, sb = c & 1;  // the group's job
-        const int block = u.two ? n >> 1 : n, kv0 = (u.j0 + block) * TR_BLOCK;
+      for (int block = u.two ? 0 : (t - blocks) & 1; block < n_blocks && ok; block += u.two ? 1 : 2, ++c) {
+        const int sb = c & 1, kv0 = (u.j0 + block) * TR_BLOCK;
         const uint32_t s_tmem = tmem_base + lane_addr + t * 128 + sb * 64;
         const uint32_t o_tmem = tmem_base + lane_addr + 256 + t * 128;
         const bool special = kv0 + TR_BLOCK > min(u.ctx, u.end);  // positions some row does not see, or that are none
@@ -610,7 +622,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         tc_fence_after_sync();
         if (active) {
           const float2 a = stats[row], b = stats[TR_ROWS + row];
-          const bool has[2] = {u.jobs > ((0 - jobs) & 1), u.jobs > ((1 - jobs) & 1)};  // the group had a job
+          const bool has[2] = {n_blocks > ((0 - blocks) & 1), n_blocks > ((1 - blocks) & 1)};  // the group had a block
           const float m = fmaxf(a.x, b.x);
           float w0 = ex2(a.x - m), w1 = ex2(b.x - m);
           const float sum = a.y * w0 + b.y * w1;
@@ -644,9 +656,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         ++joined;
         tc_fence_after_sync();
       }
-      if (u.starts && !u.whole && threadIdx.x == 64)
+      if (u.starts && !u.whole && threadIdx.x == 96)
         p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + (u.after + share - 1) / share));
-      jobs += u.jobs, blocks += u.j1 - u.j0;
+      blocks += n_blocks;
     }
   }
 
