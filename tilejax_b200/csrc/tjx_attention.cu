@@ -87,22 +87,7 @@ struct AttnSmem {
   static constexpr int TOTAL = LAST_OFF + AT_MAX_TILES * 4 + 1024;
 };
 
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// 2^x for a pair of elements. POLY: on the FMA pipe — x = n + f with n the nearest integer (the float trick of
-// adding 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f by a cubic fitted to a relative error of 7.5e-5 (P is rounded to
-// bf16, 3.9e-3, right after); n goes into the exponent field by integer addition. x below -125 is held there
-// (2^-125: nothing, after the rounding of P V and of the row sum).
+// Some of the exponentials take the FMA pipe (exp2_pair).
 #ifndef TJX_AT_POLY_PAIRS
 #define TJX_AT_POLY_PAIRS 1
 #endif
@@ -114,24 +99,6 @@ __host__ __device__ constexpr bool poly_pair(int pair) {
          : AT_POLY_PAIRS == 1 ? (pair & 3) == 3
                               : false;
 }
-__device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {  // `poly` is a constant after unrolling
-  if (!poly) {
-    return make_float2(fast_exp2(x.x), fast_exp2(x.y));
-  } else {
-    constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23
-    x.x = fmaxf(x.x, -125.f), x.y = fmaxf(x.y, -125.f);
-    const float2 t = __fadd2_rn(x, make_float2(MAGIC, MAGIC));
-    const float2 n = __fadd2_rn(t, make_float2(-MAGIC, -MAGIC));
-    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-    float2 p = __ffma2_rn(f, make_float2(0.05517164617776871f, 0.05517164617776871f),
-                          make_float2(0.2426111251115799f, 0.2426111251115799f));
-    p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
-    p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-  }
-}
-
 // Keys a slot's rows [q0, q0 + 128) attend to, as a count of 128-key sub-blocks from key 0: what the step table
 // lists for the user tile holding q0 (blocks 0 .. last, contiguous), cut at the slot's own diagonal.
 __device__ __forceinline__ int slot_blocks(const AttnParams& p, const int* last_block, int q0) {
@@ -519,7 +486,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         // Raise the running max and rescale what has been accumulated. P V of the previous block finished
         // before this block's scores were produced (the tensor pipe runs one thread's MMAs in order).
         const float m_new = fmaxf(m_used, m_blk);
-        const float alpha = fast_exp2(m_used - m_new);
+        const float alpha = ex2(m_used - m_new);
         m_used = m_new;
         l *= alpha;
         const bool od = mbar_wait(o_done(t), (done + n - 1) & 1, abort_flag, p.status, TJX_ERR_WAIT_OTHER);

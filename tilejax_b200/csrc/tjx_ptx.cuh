@@ -643,6 +643,45 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The larger of three; of a NaN and a number, the number. And the same where a NaN wins.
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// 2^x for a pair of elements. POLY: on the FMA pipe — x = n + f with n the nearest integer (the float trick of
+// adding 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f by a cubic fitted to a relative error of 7.5e-5 (P is rounded to
+// bf16, 3.9e-3, right after); n goes into the exponent field by integer addition. x below -125 is held there
+// (2^-125: nothing, after the rounding of P V and of the row sum).
+__device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {  // `poly` is a constant after unrolling
+  if (!poly) {
+    return make_float2(ex2(x.x), ex2(x.y));
+  } else {
+    constexpr float MAGIC = 12582912.f;  // 1.5 * 2^23
+    x.x = fmaxf(x.x, -125.f), x.y = fmaxf(x.y, -125.f);
+    const float2 t = __fadd2_rn(x, make_float2(MAGIC, MAGIC));
+    const float2 n = __fadd2_rn(t, make_float2(-MAGIC, -MAGIC));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(f, make_float2(0.05517164617776871f, 0.05517164617776871f),
+                          make_float2(0.2426111251115799f, 0.2426111251115799f));
+    p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+    p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  }
+}
+
 // Four 8x8 b16 matrices from shared memory: lane i gives the address of row i % 8 of matrix i / 8; register j
 // of every lane then holds, of matrix j, row lane / 4, columns 2 (lane % 4) and + 1 — or with .trans, column
 // lane / 4, rows 2 (lane % 4) and + 1.

@@ -13,7 +13,8 @@
 // one unit, whole units, and the beginning of another, and what it has of a unit that others share is a partial result
 // (running maximum, sum, unnormalised rows) that tree_join_kernel joins in order. One persistent CTA per SM:
 //
-//   warp 0      producer: TMA loads of Q (a buffer per row tile), K and V blocks (boxes of at most a page) into rings
+//   warps 0, 11 producers: TMA loads of Q (a buffer per row tile) and K blocks, and of V blocks, into rings (boxes of at
+//               most a page)
 //   warps 1, 2  MMA issuers, one for each group: S = Q K^T one job ahead of O += P V, P read from TMEM
 //   warps 3-6   softmax of the one group, warps 7-10 of the other (a thread owns a row)
 //
@@ -26,6 +27,7 @@
 // before: rings have an even number of slots and blocks keep their parity over the whole run, so that a group finds
 // its blocks in the same slots always.
 #include <algorithm>
+#include <type_traits>
 
 #include "tjx_host.cuh"
 #include "tjx_ptx.cuh"
@@ -38,8 +40,8 @@ constexpr int TR_D = 128;
 constexpr int TR_ROWS = 128;   // rows of a tile
 constexpr int TR_BLOCK = 64;   // positions of a block
 constexpr int TR_K_STAGES = 4;
-constexpr int TR_V_STAGES = 4;
-constexpr int TR_THREADS = 352;
+constexpr int TR_V_STAGES = 6;  // a V block is held longer: until its probabilities are made
+constexpr int TR_THREADS = 384;
 constexpr float TR_LOG2E = 1.4426950408889634f;
 constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a row that has seen nothing
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
@@ -55,7 +57,7 @@ struct TreeParams {
   int box_rows;    // positions of one TMA box: the largest power of two that divides the page size, at most 64
   float scale_log2e;
   int part_rows;     // rows of a partial result
-  float* part_o;     // [2 CTAs][part_rows][128]
+  float4* part_o;    // [2 CTAs][32][part_rows]: four columns of a row (a warp's rows lie side by side)
   float2* part_ml;   // [2 CTAs][part_rows]: running maximum (log2 units) and sum
   int4* joins;       // [CTAs]: the unit that starts in CTA c and ends in a later one: first token, nodes, KV head, last CTA
   int* status;
@@ -69,9 +71,10 @@ struct TreeSmem {
   static constexpr int V_OFF = K_OFF + TR_K_STAGES * KV_BYTES;
   static constexpr int STAT_OFF = V_OFF + TR_V_STAGES * KV_BYTES;  // float2[2][128]: maximum and sum of each group's rows
   static constexpr int BAD_OFF = STAT_OFF + 2 * TR_ROWS * 8;       // uint32[2 groups][2][4]: rows of V that are not finite
-  static constexpr int SCAN_OFF = BAD_OFF + 64;                    // long long[11], and where this CTA starts
-  static constexpr int BAR_OFF = SCAN_OFF + 160;
-  static constexpr int TOTAL = BAR_OFF + 512 + 1024;
+  static constexpr int SCAN_OFF = BAD_OFF + 64;                    // long long[12], and int[10]: where this CTA starts
+  static constexpr int BAR_OFF = SCAN_OFF + 96 + 40;
+  static constexpr int N_BARS = 21 + 2 * TR_K_STAGES + 2 * TR_V_STAGES;
+  static constexpr int TOTAL = BAR_OFF + 8 * N_BARS + 16;
 };
 static_assert(TR_K_STAGES % 2 == 0 && TR_V_STAGES % 2 == 0, "a slot's blocks are of one parity");
 static_assert(TreeSmem::TOTAL <= 232448, "shared memory of one CTA");
@@ -106,16 +109,6 @@ struct TreeWalk {
   int s, hk, pr, j;
   long long left;
   TreeSeq q;
-  // From block `off` of sequence s on.
-  __device__ __forceinline__ void start(const TreeParams& p, int s_, long long off, long long count) {
-    s = s_, left = count;
-    hk = pr = j = 0;
-    if (left <= 0) return;
-    load(p);
-    const int unit = static_cast<int>(off / q.blocks);
-    j = static_cast<int>(off % q.blocks);
-    hk = unit / q.pairs, pr = unit % q.pairs;
-  }
   __device__ __forceinline__ void load(const TreeParams& p) {  // by whole warps: the same values, and said to be so
     q = tree_seq(p, s);
     q.tok0 = __shfl_sync(0xFFFFFFFFu, q.tok0, 0), q.q_len = __shfl_sync(0xFFFFFFFFu, q.q_len, 0);
@@ -164,6 +157,11 @@ __device__ __forceinline__ uint32_t tree_bits(const int32_t* mask, int words, in
   return valid >= 32 ? bits : valid <= 0 ? 0u : bits & ((1u << valid) - 1u);
 }
 
+// a / b for a >= 0, b > 0: a 64-bit division only where it takes one.
+__device__ __forceinline__ long long tree_div(long long a, int b) {
+  return (a >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 __device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
   return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
 }
@@ -171,9 +169,15 @@ __device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
 __global__ void __launch_bounds__(TR_THREADS, 1)
     tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const TreeParams p) {
   using L = TreeSmem;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  extern __shared__ __align__(1024) uint8_t base_ptr[];
+  const uint32_t base = smem_u32(base_ptr);
+  if ((base & 1023u) != 0) {  // (the tiles' swizzle goes by address bits; the runtime puts the array at 1024)
+    if (threadIdx.x == 0) {
+      atomicCAS(p.status, 0, TJX_ERR_WAIT_OTHER);
+      p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
   const uint32_t bar = base + L::BAR_OFF;
   auto q_full = [&](int b) { return bar + 8u * b; };
   auto q_empty = [&](int b) { return bar + 8u * (2 + b); };
@@ -188,7 +192,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   auto k_empty = [&](int i) { return bar + 8u * (RING + TR_K_STAGES + i); };
   auto v_full = [&](int i) { return bar + 8u * (RING + 2 * TR_K_STAGES + i); };
   auto v_empty = [&](int i) { return bar + 8u * (RING + 2 * TR_K_STAGES + TR_V_STAGES + i); };
-  constexpr int N_BARS = RING + 2 * TR_K_STAGES + 2 * TR_V_STAGES;
+  constexpr int N_BARS = L::N_BARS;
+  static_assert(N_BARS == RING + 2 * TR_K_STAGES + 2 * TR_V_STAGES, "");
   volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(base_ptr + L::BAR_OFF + 8 * N_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + L::BAR_OFF + 8 * N_BARS + 8);
   volatile long long* scan = reinterpret_cast<volatile long long*>(base_ptr + L::SCAN_OFF);
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < N_BARS; ++i) {
-      // p_ready, v_seen: the warps of a group; the next three: of both. A Q, K or V buffer is free when both issuers say
+      // p_ready, v_seen: the warps of a group; the next three: of both. A Q, K or V buffer is free when both groups say
       // so (where only one uses it, the producer speaks for the other).
       const bool by_both = i == 2 || i == 3 || (i >= RING + TR_K_STAGES && i < RING + 2 * TR_K_STAGES) ||
                            i >= RING + 2 * TR_K_STAGES + TR_V_STAGES;
@@ -215,16 +220,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     tmem_relinquish();
   }
   // All blocks counted, and where this CTA's run starts: a thread takes consecutive sequences, the thread that has the
-  // run's first block finds its sequence.
-  const int seqs = min(max(p.distribution[0], 0), p.S);
-  const int per_thread = (seqs + TR_THREADS - 1) / TR_THREADS;
-  auto blocks_of = [&](int s) {
-    const TreeSeq q = tree_seq(p, s);
-    return static_cast<long long>(q.blocks) * q.pairs * p.Hkv;
-  };
-  const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, seqs), s_hi = min(s_lo + per_thread, seqs);
+  // run's first block finds its sequence. (The lengths are read without waiting for the number of sequences.)
+  volatile int* start = reinterpret_cast<volatile int*>(base_ptr + L::SCAN_OFF + 96);
+  const int per_thread = (p.S + TR_THREADS - 1) / TR_THREADS;
+  const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, p.S), s_hi = min(s_lo + per_thread, p.S);
+  const int distribution = p.distribution[0];
+  auto blocks_of = [&](const TreeSeq& q) { return static_cast<long long>(q.blocks) * (q.pairs * static_cast<long long>(p.Hkv)); };
   long long mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += blocks_of(s);
+  for (int s = s_lo; s < s_hi; ++s) {
+    const long long n = blocks_of(tree_seq(p, s));
+    mine += s < distribution ? n : 0;
+  }
   long long upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -239,33 +245,46 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     if (w == warp) upto += total;
     total += scan[w];
   }
-  const long long share = max((total + gridDim.x - 1) / static_cast<long long>(gridDim.x), static_cast<long long>(TR_MIN_SHARE));
+  const long long share = max(tree_div(total + gridDim.x - 1, gridDim.x), static_cast<long long>(TR_MIN_SHARE));
   const long long first = share * blockIdx.x, count = min(share, total - first);  // (count <= 0: nothing)
   if (count > 0 && first >= upto - mine && first < upto) {
     long long off = first - (upto - mine);
     int s = s_lo;
-    for (long long n; off >= (n = blocks_of(s)); ++s) off -= n;
-    scan[11] = s, scan[12] = off;
+    TreeSeq q = tree_seq(p, s);
+    for (long long n; off >= (n = blocks_of(q)); q = tree_seq(p, ++s)) off -= n;
+    const int unit = static_cast<int>(tree_div(off, q.blocks));
+    start[0] = s, start[1] = unit / q.pairs, start[2] = unit % q.pairs;
+    start[3] = static_cast<int>(off - static_cast<long long>(unit) * q.blocks);
+    start[4] = q.tok0, start[5] = q.q_len, start[6] = q.ctx, start[7] = q.end, start[8] = q.blocks, start[9] = q.pairs;
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   chain_release();
   const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
+  // (Through shuffles: the compiler must know that a warp's lanes walk together, or it keeps the issuers' addresses and
+  // loop counters per lane.)
   TreeWalk walk;
-  walk.start(p, __shfl_sync(0xFFFFFFFFu, static_cast<int>(scan[11]), 0), __shfl_sync(0xFFFFFFFFu, scan[12], 0), count);
+  {
+    const int word = lane < 10 ? start[lane] : 0;
+    auto get = [&](int i) { return __shfl_sync(0xFFFFFFFFu, word, i); };
+    walk.s = get(0), walk.hk = get(1), walk.pr = get(2), walk.j = get(3);
+    walk.q.tok0 = get(4), walk.q.q_len = get(5), walk.q.ctx = get(6), walk.q.end = get(7), walk.q.blocks = get(8);
+    walk.q.pairs = get(9), walk.left = __shfl_sync(0xFFFFFFFFu, count, 0);
+  }
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ producer
+  if (warp == 0 || warp == 11) {
+    // ------------------------------------------------------------------ producers: of Q and K, of V
+    const bool keys = warp == 0;
     bool ok = true;
-    int qc = 0;  // Q tiles loaded so far
-    int ks = 0, vs = 0;
-    uint32_t kph = 0, vph = 0;
+    int qc = 0;      // Q tiles loaded so far
+    int block = 0;   // blocks loaded so far
     const int boxes = TR_BLOCK / p.box_rows;
     const uint32_t box_bytes = p.box_rows * 128;
     // Lane l loads half l % 2 (64 columns) of box l / 2.
     const int box = lane >> 1, half = lane & 1;
     const bool loads = lane < 2 * boxes;
+    const uint32_t lane_off = half * (L::KV_BYTES / 2) + box * box_bytes;
     auto wait = [&](uint32_t b, uint32_t parity) {
       return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, TJX_ERR_WAIT_EMPTY)) != 0;
     };
@@ -281,41 +300,37 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         return min(max(page, 0), p.num_pages - 1) * p.page_size + (pos - entry * p.page_size);
       };
       int next_row = loads ? cache_row(u.j0) : 0;
-      for (int r = 0; r < (u.two ? 2 : 1) && ok; ++r, ++qc) {
-        const int b = qc & 1;
-        ok = wait(q_empty(b), ((qc >> 1) & 1) ^ 1u);
-        if (!ok) break;
-        if (lane == 0) {
-          const uint32_t dst = base + L::Q_OFF + b * L::Q_BYTES;
-          mbar_expect_tx(q_full(b), static_cast<uint32_t>(p.tile_nodes * p.group) * 256u);
-          const int tok = u.tok + r * p.tile_nodes;
-          tma_load_3d(dst, &map_q, 0, u.hk * p.group, tok, q_full(b));
-          tma_load_3d(dst + L::Q_BYTES / 2, &map_q, 64, u.hk * p.group, tok, q_full(b));
-          if (u.two) mbar_arrive(q_empty(b));  // one issuer uses it
+      if (keys) {
+        for (int r = 0; r < (u.two ? 2 : 1) && ok; ++r, ++qc) {
+          const int b = qc & 1;
+          ok = wait(q_empty(b), ((qc >> 1) & 1) ^ 1u);
+          if (!ok) break;
+          if (lane == 0) {
+            const uint32_t dst = base + L::Q_OFF + b * L::Q_BYTES;
+            mbar_expect_tx(q_full(b), static_cast<uint32_t>(p.tile_nodes * p.group) * 256u);
+            const int tok = u.tok + r * p.tile_nodes;
+            tma_load_3d(dst, &map_q, 0, u.hk * p.group, tok, q_full(b));
+            tma_load_3d(dst + L::Q_BYTES / 2, &map_q, 64, u.hk * p.group, tok, q_full(b));
+            if (u.two) mbar_arrive(q_empty(b));  // one group uses it
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
-      for (int j = u.j0; j < u.j1 && ok; ++j) {
+      for (int j = u.j0; j < u.j1 && ok; ++j, ++block) {
         const int row = next_row;
         if (loads && j + 1 < u.j1) next_row = cache_row(j + 1);
-        ok = wait(k_empty(ks), kph ^ 1u);
+        const int slot = block % (keys ? TR_K_STAGES : TR_V_STAGES), use = block / (keys ? TR_K_STAGES : TR_V_STAGES);
+        const uint32_t full = keys ? k_full(slot) : v_full(slot), empty = keys ? k_empty(slot) : v_empty(slot);
+        ok = wait(empty, (use & 1) ^ 1u);
         if (!ok) break;
-        if (lane == 0) mbar_expect_tx(k_full(ks), L::KV_BYTES);
+        if (lane == 0) {
+          mbar_expect_tx(full, L::KV_BYTES);
+          if (!u.two) mbar_arrive(empty);
+        }
         __syncwarp();
         if (loads)
-          tma_load_3d(base + L::K_OFF + ks * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
-                      2 * u.hk, row, k_full(ks));
-        if (lane == 0 && !u.two) mbar_arrive(k_empty(ks));
-        if (++ks == TR_K_STAGES) ks = 0, kph ^= 1u;
-        ok = wait(v_empty(vs), vph ^ 1u);
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(v_full(vs), L::KV_BYTES);
-        __syncwarp();
-        if (loads)
-          tma_load_3d(base + L::V_OFF + vs * L::KV_BYTES + half * (L::KV_BYTES / 2) + box * box_bytes, &map_kv, 64 * half,
-                      2 * u.hk + 1, row, v_full(vs));
-        if (lane == 0 && !u.two) mbar_arrive(v_empty(vs));
-        if (++vs == TR_V_STAGES) vs = 0, vph ^= 1u;
+          tma_load_3d(base + (keys ? L::K_OFF : L::V_OFF) + slot * L::KV_BYTES + lane_off, &map_kv, 64 * half,
+                      2 * u.hk + (keys ? 0 : 1), row, full);
       }
     }
     __syncwarp();
@@ -364,7 +379,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           kd[kk] = k0 + (((kk >> 2) * (L::KV_BYTES / 2) + (kk & 3) * 32) >> 4);
         }
         mma_ss_x8_commit(tmem_base + t * 128 + (ca & 1) * 64, qd, kd, idesc_qk, 0u, s_full(t, ca & 1));
-        mma_commit_elected(k_empty(ks));
         ia += a.two ? 1 : 2, ++ca;
         if (ia >= a.j1 - a.j0) mma_commit_elected(q_empty(q_buffer));  // this group's last use of the tile
       }
@@ -469,6 +483,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         ok = wait(s_full(t, sb), (c >> 1) & 1, TJX_ERR_WAIT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after_sync();
+        // The scores are there, so the block's keys have been read. (An arrival here is cheaper than the issuer's commit.)
+        if (quarter == 0 && lane == 0) mbar_arrive(k_empty((blocks + block) % TR_K_STAGES));
         uint32_t pk[32];
         uint32_t see[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         if (active) {
@@ -491,12 +507,16 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[h][i]));
-          const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
+            for (int i = 0; i < 32; i += 2)
+              mx[(i >> 1) & 3] = fmax3_nan(mx[(i >> 1) & 3], __uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1]));
+          // A score that is NaN or infinite makes the row NaN, as the formula does: through the maximum, since not every
+          // way to an exponential keeps a NaN.
+          float m_blk = fmax_nan(fmax3_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2e;
+          if (m_blk == INFINITY) m_blk = NAN;
           if (last_job < 0) {
-            m_used = fmaxf(m_blk, TR_NOTHING);
-          } else if (__any_sync(0xFFFFFFFFu, m_blk > m_used + TR_RESCALE)) {
-            const float m_new = fmaxf(m_used, m_blk), alpha = ex2(m_used - m_new);
+            m_used = fmax_nan(m_blk, TR_NOTHING);
+          } else if (__any_sync(0xFFFFFFFFu, !(m_blk <= m_used + TR_RESCALE))) {
+            const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
             ok = output_done(c - 1);
@@ -514,18 +534,26 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             tmem_wait_st();
           }
           // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention);
-          // the sum adds the unrounded values.
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // the sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA
+          // pipe, but where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0).
+          const float2 scale = make_float2(p.scale_log2e, p.scale_log2e), neg_m = make_float2(-m_used, -m_used);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          auto weights = [&](auto poly) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(v[h][i]), p.scale_log2e, -m_used));
-              const float e1 = ex2(fmaf(__uint_as_float(v[h][i + 1]), p.scale_log2e, -m_used));
-              sum[(i >> 1) & 1] += e0, sum[2 + ((i >> 1) & 1)] += e1;
-              pk[h * 16 + (i >> 1)] = pack_bf16(e0, e1);
-            }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+              for (int i = 0; i < 32; i += 2) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1])), scale, neg_m);
+                const float2 e = exp2_pair(x, poly.value && (i & 6) == 6);
+                sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], e);
+                pk[h * 16 + (i >> 1)] = pack_bf16(e.x, e.y);
+              }
+          };
+          if (special)
+            weights(std::false_type{});
+          else
+            weights(std::true_type{});
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_st32(s_tmem, pk);
           tmem_wait_st();
         }
@@ -578,21 +606,46 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       if (!ok) break;
       const int part = 2 * blockIdx.x + (u.starts ? 1 : 0);
       const int head = u.hk * p.group + row - node * p.group;
-      const size_t out_row = static_cast<size_t>(tok) * p.H + head;
-      const size_t part_row = static_cast<size_t>(part) * p.part_rows + tile * p.tile_nodes * p.group + row;
-      auto store32 = [&](int col, const float (&o)[32]) {  // 32 columns of this thread's row
+      const size_t part_row = static_cast<size_t>(part) * 32 * p.part_rows + tile * p.tile_nodes * p.group + row;
+      // 32 columns from `col` on of every row of the warp (all lanes call it).
+      int out_rows[4];  // the rows of the lane's group of four, -1: none
+      {
+        const int out_row = mine_valid ? tok * p.H + head : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out_rows[k] = __shfl_sync(0xFFFFFFFFu, out_row, (lane & ~3) + k);
+      }
+      auto store32 = [&](int col, const float (&o)[32]) {
         if (u.whole) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + out_row * TR_D + col);
+          // Four lanes hold 64 bytes of four rows: they exchange 16-byte pieces, so that a store instruction writes 64
+          // bytes of eight rows, not 16 of 32 (each row is a line of its own).
+          uint32_t w[4][4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            dst[x] = make_uint4(pack_bf16(o[8 * x], o[8 * x + 1]), pack_bf16(o[8 * x + 2], o[8 * x + 3]),
-                                pack_bf16(o[8 * x + 4], o[8 * x + 5]), pack_bf16(o[8 * x + 6], o[8 * x + 7]));
-        } else {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + part_row * TR_D + col);
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) dst[x] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            for (int x = 0; x < 4; ++x) w[k][x] = pack_bf16(o[8 * k + 2 * x], o[8 * k + 2 * x + 1]);
+#pragma unroll
+          for (int d = 1; d <= 2; d <<= 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (k & d) continue;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, (lane & d) ? w[k][x] : w[k + d][x], d);
+                if (lane & d) w[k][x] = got; else w[k + d][x] = got;
+              }
+            }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (out_rows[k] >= 0)
+              reinterpret_cast<uint4*>(p.out + static_cast<size_t>(out_rows[k]) * TR_D + col)[lane & 3] =
+                  make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        } else if (mine_valid) {
+          float4* dst = p.part_o + part_row + static_cast<size_t>(col / 4) * p.part_rows;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) dst[x * p.part_rows] = make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
         }
       };
+      const size_t ml_row = static_cast<size_t>(part) * p.part_rows + tile * p.tile_nodes * p.group + row;
       if (u.two) {
         tc_fence_after_sync();
         const float inv = u.whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
@@ -605,9 +658,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             float f[32];
 #pragma unroll
             for (int x = 0; x < 32; ++x) f[x] = __uint_as_float(o[x]) * inv;
-            if (mine_valid) store32(i * 32, f);
+            store32(i * 32, f);
           }
-          if (mine_valid && !u.whole) p.part_ml[part_row] = make_float2(m_used, l);
+          if (mine_valid && !u.whole) p.part_ml[ml_row] = make_float2(m_used, l);
         }
         tc_fence_before_sync();
       } else {
@@ -645,9 +698,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
               for (int x = 0; x < 32; ++x) f[x] = fmaf(__uint_as_float(o[x]), w, f[x]);
             }
-            if (mine_valid) store32(i * 32, f);
+            store32(i * 32, f);
           }
-          if (mine_valid && !u.whole && t == 0) p.part_ml[part_row] = make_float2(m, sum);
+          if (mine_valid && !u.whole && t == 0) p.part_ml[ml_row] = make_float2(m, sum);
         }
         tc_fence_before_sync();
         __syncwarp();
@@ -671,46 +724,41 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   }
 }
 
-constexpr int TJ_WARPS = 8;  // rows of a CTA
+constexpr int TJ_WARPS = 8;
 
-// The units that several CTAs shared: a warp per row joins its partial results in the order of the blocks. And the rows
-// that no unit has, which stay the query.
+// The units that several CTAs shared: a CTA per 32 rows (a lane's) joins their partial results in the order of the
+// blocks, a warp 16 of the columns. And the rows that no unit has, which stay the query.
 __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
   chain_wait();
-  const int lane = threadIdx.x & 31, x = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = blockIdx.y * 32 + lane;
   const int4 join = p.joins[blockIdx.x];
   if (x < join.y * p.group) {
     const int first = blockIdx.x, n = join.w - first + 1;  // parts: 2 first + 1, 2 (first + 1), 2 (first + 2), ...
-    auto part_row = [&](int i) {
-      return static_cast<size_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.part_rows + x;
-    };
+    auto part = [&](int i) { return static_cast<size_t>(2 * (first + i) + (i == 0 ? 1 : 0)); };
     float m = TR_NOTHING;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[part_row(i)].x);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    float sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      float w = 0.f;
-      if (i0 + lane < n) {
-        const float2 ml = p.part_ml[part_row(i0 + lane)];
-        w = ex2(ml.x - m);
-        sum += w * ml.y;
-      }
-      const int some = min(n - i0, 32);
 #pragma unroll 4
-      for (int i = 0; i < some; ++i) {
-        const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
-        const float4 v = reinterpret_cast<const float4*>(p.part_o + part_row(i0 + i) * TR_D)[lane];
-        o.x = fmaf(v.x, wi, o.x), o.y = fmaf(v.y, wi, o.y), o.z = fmaf(v.z, wi, o.z), o.w = fmaf(v.w, wi, o.w);
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.part_ml[part(i) * p.part_rows + x].x);
+    float sum = 0.f, o[16] = {};
+#pragma unroll 2
+    for (int i = 0; i < n; ++i) {
+      const float2 ml = p.part_ml[part(i) * p.part_rows + x];
+      const float w = ex2(ml.x - m);
+      sum = fmaf(w, ml.y, sum);
+      const float4* src = p.part_o + (part(i) * 32 + 4 * warp) * p.part_rows + x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = src[static_cast<size_t>(k) * p.part_rows];
+        o[4 * k] = fmaf(v.x, w, o[4 * k]), o[4 * k + 1] = fmaf(v.y, w, o[4 * k + 1]);
+        o[4 * k + 2] = fmaf(v.z, w, o[4 * k + 2]), o[4 * k + 3] = fmaf(v.w, w, o[4 * k + 3]);
       }
     }
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     const size_t row = static_cast<size_t>(join.x + x / p.group) * p.H + join.z * p.group + x % p.group;
-    reinterpret_cast<uint2*>(p.out + row * TR_D)[lane] =
-        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    uint4* dst = reinterpret_cast<uint4*>(p.out + row * TR_D + 16 * warp);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      dst[k] = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                          pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
   }
   if (p.out != p.q) {
     const int seqs = min(max(p.distribution[0], 0), p.S);
@@ -783,7 +831,7 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.joins = reinterpret_cast<int4*>(w), w += tree_align256(ctas * sizeof(int4));
   p.part_ml = reinterpret_cast<float2*>(w), w += tree_align256(2ull * ctas * p.part_rows * sizeof(float2));
-  p.part_o = reinterpret_cast<float*>(w);
+  p.part_o = reinterpret_cast<float4*>(w);
 
   CUtensorMap mq, mkv;
   {
@@ -810,6 +858,6 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   tree_kernel<<<ctas, TR_THREADS, TreeSmem::TOTAL, s>>>(mq, mkv, p);
   TJX_CUDA(cudaGetLastError());
-  TJX_CUDA(launch_chained(tree_join_kernel, dim3(ctas, (p.part_rows + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, s, p));
+  TJX_CUDA(launch_chained(tree_join_kernel, dim3(ctas, (p.part_rows + 31) / 32), dim3(TJ_WARPS * 32), 0, s, p));
   return 0;
 }
