@@ -201,17 +201,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   volatile uint32_t* bad_rows = reinterpret_cast<volatile uint32_t*>(base_ptr + L::BAD_OFF);
 
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < N_BARS; ++i) {
-      // p_ready, v_seen: the warps of a group; the next three: of both. A Q, K or V buffer is free when both groups say
-      // so (where only one uses it, the producer speaks for the other).
-      const bool by_both = i == 2 || i == 3 || (i >= RING + TR_K_STAGES && i < RING + 2 * TR_K_STAGES) ||
-                           i >= RING + 2 * TR_K_STAGES + TR_V_STAGES;
-      const int arrivals = (i >= 8 && i < 12) || i == 16 || i == 17 ? 4 : i >= 18 && i < RING ? 8 : by_both ? 2 : 1;
-      mbar_init(bar + 8u * i, arrivals);
-    }
-    *abort_flag = 0;
+  if (threadIdx.x < N_BARS) {
+    // p_ready, v_seen: the warps of a group; the next three: of both. A Q, K or V buffer is free when both groups say
+    // so (where only one uses it, the producer speaks for the other).
+    const int i = threadIdx.x;
+    const bool by_both = i == 2 || i == 3 || (i >= RING + TR_K_STAGES && i < RING + 2 * TR_K_STAGES) ||
+                         i >= RING + 2 * TR_K_STAGES + TR_V_STAGES;
+    mbar_init(bar + 8u * i, (i >= 8 && i < 12) || i == 16 || i == 17 ? 4 : i >= 18 && i < RING ? 8 : by_both ? 2 : 1);
     mbar_fence_init();
+  }
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_kv);
   }
@@ -227,9 +227,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   const int distribution = p.distribution[0];
   auto blocks_of = [&](const TreeSeq& q) { return static_cast<long long>(q.blocks) * (q.pairs * static_cast<long long>(p.Hkv)); };
   long long mine = 0;
+  TreeSeq q_lo{};
   for (int s = s_lo; s < s_hi; ++s) {
-    const long long n = blocks_of(tree_seq(p, s));
-    mine += s < distribution ? n : 0;
+    const TreeSeq q = tree_seq(p, s);
+    if (s == s_lo) q_lo = q;
+    mine += s < distribution ? blocks_of(q) : 0;
   }
   long long upto = mine;
 #pragma unroll
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   if (count > 0 && first >= upto - mine && first < upto) {
     long long off = first - (upto - mine);
     int s = s_lo;
-    TreeSeq q = tree_seq(p, s);
+    TreeSeq q = q_lo;
     for (long long n; off >= (n = blocks_of(q)); q = tree_seq(p, ++s)) off -= n;
     const int unit = static_cast<int>(tree_div(off, q.blocks));
     start[0] = s, start[1] = unit / q.pairs, start[2] = unit % q.pairs;
@@ -291,15 +293,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     TreePortion u;
     while (ok && walk.next(p, u)) {
       const int32_t* table = p.page_indices + static_cast<size_t>(u.s) * p.pages_per_seq;
-      // Row of the cache (page * page_size + row) where this lane's box of block j starts. (An entry past the table or
-      // a page past the pool is clamped, as a gather's index is.)
-      auto cache_row = [&](int j) {
+      // The page of this lane's box of block j, and the box's first row there: fetched a block ahead. (An entry past the
+      // table or a page past the pool is clamped, as a gather's index is.)
+      int page = 0, page_row = 0;
+      auto fetch = [&](int j) {
         const int pos = j * TR_BLOCK + box * p.box_rows;
         const int entry = pos / p.page_size;
-        const int page = table[min(entry, p.pages_per_seq - 1)];
-        return min(max(page, 0), p.num_pages - 1) * p.page_size + (pos - entry * p.page_size);
+        page = table[min(entry, p.pages_per_seq - 1)], page_row = pos - entry * p.page_size;
       };
-      int next_row = loads ? cache_row(u.j0) : 0;
+      if (loads) fetch(u.j0);
       if (keys) {
         for (int r = 0; r < (u.two ? 2 : 1) && ok; ++r, ++qc) {
           const int b = qc & 1;
@@ -317,8 +319,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
       }
       for (int j = u.j0; j < u.j1 && ok; ++j, ++block) {
-        const int row = next_row;
-        if (loads && j + 1 < u.j1) next_row = cache_row(j + 1);
+        const int row = min(max(page, 0), p.num_pages - 1) * p.page_size + page_row;
+        if (loads && j + 1 < u.j1) fetch(j + 1);
         const int slot = block % (keys ? TR_K_STAGES : TR_V_STAGES), use = block / (keys ? TR_K_STAGES : TR_V_STAGES);
         const uint32_t full = keys ? k_full(slot) : v_full(slot), empty = keys ? k_empty(slot) : v_empty(slot);
         ok = wait(empty, (use & 1) ^ 1u);
@@ -566,15 +568,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           ok = output_done(c);
           if (!ok) break;
           tc_fence_after_sync();
+          volatile uint32_t weights_of[32];  // (indexed below: a copy, or P itself would live in local memory in every block)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) weights_of[i] = pk[i];
 #pragma unroll 1
           for (int g = 0; g < TR_BLOCK; ++g) {
             const uint32_t some = g < 32 ? (g < 16 ? bad[0] : bad[1]) : (g < 48 ? bad[2] : bad[3]);
             if (!((some >> (2 * (g & 15))) & 1)) continue;
             const bool sees = ((g < 32 ? see[0] : see[1]) >> (g & 31)) & 1;
-            uint32_t pair = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i == g >> 1) pair = pk[i];
+            const uint32_t pair = weights_of[g >> 1];
             const float weight = (g & 1) ? bf16_hi(pair) : bf16_lo(pair);
             const int pos = kv0 + g;  // (below the end)
             const int page = min(max(p.page_indices[static_cast<size_t>(u.s) * p.pages_per_seq + pos / p.page_size], 0), p.num_pages - 1);
