@@ -207,12 +207,12 @@ def tree_case(q_lens, kv_lens, heads, kv_heads, page_size, *, words=None, max_se
                 tree_mask=np.concatenate(masks), distribution=np.array([len(q_lens)] * 3, np.int32))
 
 
-def check_tree(inp, sm_scale=128**-0.5):
+def check_tree(inp, sm_scale=128**-0.5, slack=2.0**-8 + 2.0**-11):
     dev = {k: to_device(v) for k, v in inp.items()}
     got = ops.rpa_tree_attention(**dev, sm_scale=sm_scale)
     assert ops.device_status() == 0
     want, size = oracle.tree_attention_f64(*inp.values(), sm_scale)
-    close(to_host(got), want, size, 2.0**-8 + 2.0**-11)
+    close(to_host(got), want, size, slack)
     np.testing.assert_array_equal(to_host(dev["q"]).view(np.uint16), inp["q"].view(np.uint16))
     rest = int(inp["cu_q_lens"][inp["distribution"][0]])
     np.testing.assert_array_equal(to_host(got)[rest:].view(np.uint16), inp["q"][rest:].view(np.uint16))
@@ -296,6 +296,20 @@ def test_runs_of_many_units_and_units_of_many_runs(heads, kv_heads, page, seqs, 
     for _ in range(20):  # the same bits every time
         assert torch.equal(ops.rpa_tree_attention(**dev, sm_scale=128**-0.5).view(torch.int16), first.view(torch.int16))
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("rising", [False, True])
+def test_scores_hundreds_apart(rising):
+    # Scores whose exponentials leave f32's range unless the running maximum follows. f32's error in a score is at most
+    # 128 * 2^-24 of the sum of |q k| (about 128 * 200 * 0.64) times the scale: 0.011, the weights' relative error: 2^-5
+    # is well above twice that and the roundings to bf16.
+    inp = tree_case([9, 16, 40], [700, 90, 333], 8, 2, 16, scale=200.0, seed=7)
+    if rising:  # later positions have larger keys
+        for s, n in enumerate(inp["kv_lens"]):
+            pages = inp["page_indices"].reshape(3, -1)[s, : -(-n // 16)]
+            growth = np.linspace(0.01, 1.0, len(pages), dtype=np.float32)[:, None, None, None]
+            inp["kv_cache"][pages, :, :, 0] = (inp["kv_cache"][pages, :, :, 0].astype(np.float32) * growth).astype(BF16)
+    check_tree(inp, slack=2.0**-5)
 
 
 def test_a_longer_tree_than_its_cache_and_lengths_past_the_table():

@@ -9,9 +9,10 @@
 // 5.8 of its tensor rate. So one kernel serves one node and many: whole 128-row tcgen05 tiles, padded.
 //
 // A unit is (sequence, KV head, up to 256 rows): its rows make one tile of 128, or two that share every K / V block of
-// 64 positions. The blocks of all units, in order, are cut into equal runs, one for each CTA: a CTA walks the end of
-// one unit, whole units, and the beginning of another, and what it has of a unit that others share is a partial result
-// (running maximum, sum, unnormalised rows) that tree_join_kernel joins in order. One persistent CTA per SM:
+// 64 positions. The units' blocks, in order and weighed by what they cost, are cut into equal runs, one for each CTA: a
+// CTA walks the end of one unit, whole units, and the beginning of another, and what it has of a unit that others share
+// is a partial result (running maximum, sum, unnormalised rows) that tree_join_kernel joins in order. One persistent CTA
+// per SM:
 //
 //   warps 0, 11 producers: TMA loads of Q (a buffer per row tile) and K blocks, and of V blocks, into rings (boxes of at
 //               most a page)
@@ -45,7 +46,13 @@ constexpr int TR_THREADS = 384;
 constexpr float TR_LOG2E = 1.4426950408889634f;
 constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a row that has seen nothing
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
-constexpr int TR_MIN_SHARE = 4;       // blocks of a CTA's run, at least
+// What a run is cut by, in units of about 300 cycles: a block of one row tile (bound by its loads, 1230 cycles), of two
+// (by their softmax, 1950), and what a unit takes beside its blocks: the last scores masked and their V rows looked at, the
+// pipeline drained, the rows out. Without the weights the CTA with the most units, or with the widest, ran a third longer
+// than the others (trees of 16 over 32 caches of up to 4096: 81 -> 66 us; of up to 64 over 64 of up to 8100: 340 -> 311).
+constexpr int TR_COST_ONE = 4, TR_COST_TWO = 6, TR_COST_UNIT = 24;
+constexpr int TR_MIN_SHARE = 12;  // a run's cost, at least (it may not be shorter than a block)
+static_assert(TR_MIN_SHARE >= TR_COST_TWO && TR_MIN_SHARE >= TR_COST_ONE, "every run inside a unit has a block");
 
 struct TreeParams {
   const __nv_bfloat16* q;
@@ -95,19 +102,37 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
   return r;
 }
 
-// A CTA's walk over its run of blocks: the same in every role.
+// a / b for a >= 0, b > 0: a 64-bit division only where it takes one.
+__device__ __forceinline__ long long tree_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// What the units of one KV head of a sequence cost, and one unit of two row tiles.
+__device__ __forceinline__ long long tree_pair_cost(const TreeSeq& q) {
+  return TR_COST_UNIT + static_cast<long long>(q.blocks) * TR_COST_TWO;
+}
+__device__ __forceinline__ int tree_block_cost(const TreeParams& p, const TreeSeq& q, int pr) {
+  return q.q_len - pr * 2 * p.tile_nodes > p.tile_nodes ? TR_COST_TWO : TR_COST_ONE;
+}
+__device__ __forceinline__ long long tree_head_cost(const TreeParams& p, const TreeSeq& q) {
+  return q.pairs == 0 ? 0
+                      : (q.pairs - 1) * tree_pair_cost(q) + TR_COST_UNIT +
+                            static_cast<long long>(q.blocks) * tree_block_cost(p, q, q.pairs - 1);
+}
+
+// A CTA's walk over its run: the same in every role. Block j of a unit costs its weight from TR_COST_UNIT + j * weight
+// on and is of the run that this falls into.
 struct TreePortion {
   int s, tok, nodes;     // first token and nodes of the unit
   int hk, ctx, end;
-  int node0;             // (first node's index in its sequence)
   int j0, j1;            // blocks of the unit
   bool whole, starts;    // all of the unit's blocks; its first block among them
   bool two;              // two row tiles
-  long long after;       // blocks of the unit behind this portion
+  long long past;        // where the unit's last block starts, seen from the end of the run
 };
 struct TreeWalk {
-  int s, hk, pr, j;
-  long long left;
+  int s, hk, pr;
+  long long at, left;  // of the unit's cost, where the walk stands; of the run's, what is left
   TreeSeq q;
   __device__ __forceinline__ void load(const TreeParams& p) {  // by whole warps: the same values, and said to be so
     q = tree_seq(p, s);
@@ -116,50 +141,57 @@ struct TreeWalk {
     q.blocks = __shfl_sync(0xFFFFFFFFu, q.blocks, 0), q.pairs = __shfl_sync(0xFFFFFFFFu, q.pairs, 0);
   }
   __device__ __forceinline__ bool next(const TreeParams& p, TreePortion& o) {
-    if (left <= 0) return false;
-    const int take = static_cast<int>(min(static_cast<long long>(q.blocks - j), left));
-    o.s = s, o.hk = hk, o.ctx = q.ctx, o.end = q.end;
-    o.node0 = pr * 2 * p.tile_nodes;
-    o.tok = q.tok0 + o.node0;
-    o.nodes = min(q.q_len - o.node0, 2 * p.tile_nodes);
-    o.two = o.nodes > p.tile_nodes;
-    o.j0 = j, o.j1 = j + take;
-    o.starts = j == 0, o.whole = o.starts && o.j1 == q.blocks;
-    o.after = q.blocks - o.j1;
-    left -= take, j += take;
-    if (j == q.blocks) {
-      j = 0;
+    while (left > 0) {
+      const int weight = tree_block_cost(p, q, pr), node0 = pr * 2 * p.tile_nodes;
+      const long long cost = TR_COST_UNIT + static_cast<long long>(q.blocks) * weight, to = at + left;
+      o.s = s, o.hk = hk, o.ctx = q.ctx, o.end = q.end;
+      o.tok = q.tok0 + node0;
+      o.nodes = min(q.q_len - node0, 2 * p.tile_nodes);
+      o.two = o.nodes > p.tile_nodes;
+      o.j0 = at <= TR_COST_UNIT ? 0 : static_cast<int>(tree_div(at - TR_COST_UNIT + weight - 1, weight));
+      o.j1 = to >= cost ? q.blocks : to <= TR_COST_UNIT ? 0 : static_cast<int>(tree_div(to - TR_COST_UNIT + weight - 1, weight));
+      o.starts = o.j0 == 0, o.whole = o.starts && o.j1 == q.blocks;
+      o.past = cost - weight - to;
+      left = to - cost, at = 0;
       if (++pr == q.pairs) {
         pr = 0;
         if (++hk == p.Hkv) {
           hk = 0;
           if (left > 0) {
-            do ++s, load(p); while (q.pairs == 0);  // (blocks are left, so a sequence with some follows)
+            do ++s, load(p); while (q.pairs == 0);  // (something is left, so a sequence with a unit follows)
           }
         }
       }
+      if (o.j1 > o.j0) return true;
     }
-    return true;
+    return false;
   }
 };
 
 // 32 positions from `pos` on as a row sees them: its mask's bits from node pos - ctx on, ones before the first node,
 // zeros past the mask's words and from `end` on.
-__device__ __forceinline__ uint32_t tree_bits(const int32_t* mask, int words, int pos, int ctx, int end) {
+struct TreeMask {  // a row's mask, its first two words fetched ahead
+  const int32_t* row;
+  int words;
+  uint32_t first, second;
+  __device__ __forceinline__ uint32_t word(int w) const {
+    return w < 0 ? 0xFFFFFFFFu : w == 0 ? first : w == 1 ? second : w < words ? static_cast<uint32_t>(row[w]) : 0u;
+  }
+};
+__device__ __forceinline__ uint32_t tree_bits(const TreeMask& mask, int pos, int ctx, int end) {
   uint32_t bits = 0xFFFFFFFFu;
   if (pos + 32 > ctx) {
     const int o = pos - ctx, w = o >> 5, shift = o & 31;  // (arithmetic shift: w = -1 or less before the nodes)
-    const uint32_t lo = w < 0 ? 0xFFFFFFFFu : w < words ? static_cast<uint32_t>(mask[w]) : 0u;
-    const uint32_t hi = w + 1 < 0 ? 0xFFFFFFFFu : w + 1 < words ? static_cast<uint32_t>(mask[w + 1]) : 0u;
-    bits = __funnelshift_r(lo, hi, shift);
+    bits = __funnelshift_r(mask.word(w), mask.word(w + 1), shift);
   }
   const int valid = end - pos;
   return valid >= 32 ? bits : valid <= 0 ? 0u : bits & ((1u << valid) - 1u);
 }
 
-// a / b for a >= 0, b > 0: a 64-bit division only where it takes one.
-__device__ __forceinline__ long long tree_div(long long a, int b) {
-  return (a >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+// A whole warp's bounded wait, with one outcome for all lanes; a phase that is there already costs one test and one vote.
+__device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__builtin_expect(__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity) != 0), 1)) return true;
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
 }
 
 __device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
@@ -219,19 +251,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_holder)), 512);
     tmem_relinquish();
   }
-  // All blocks counted, and where this CTA's run starts: a thread takes consecutive sequences, the thread that has the
+  // All costs added up, and where this CTA's run starts: a thread takes consecutive sequences, the thread that has the
   // run's first block finds its sequence. (The lengths are read without waiting for the number of sequences.)
   volatile int* start = reinterpret_cast<volatile int*>(base_ptr + L::SCAN_OFF + 96);
   const int per_thread = (p.S + TR_THREADS - 1) / TR_THREADS;
   const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, p.S), s_hi = min(s_lo + per_thread, p.S);
   const int distribution = p.distribution[0];
-  auto blocks_of = [&](const TreeSeq& q) { return static_cast<long long>(q.blocks) * (q.pairs * static_cast<long long>(p.Hkv)); };
+  auto cost_of = [&](const TreeSeq& q) { return tree_head_cost(p, q) * p.Hkv; };
   long long mine = 0;
   TreeSeq q_lo{};
   for (int s = s_lo; s < s_hi; ++s) {
     const TreeSeq q = tree_seq(p, s);
     if (s == s_lo) q_lo = q;
-    mine += s < distribution ? blocks_of(q) : 0;
+    mine += s < distribution ? cost_of(q) : 0;
   }
   long long upto = mine;
 #pragma unroll
@@ -253,10 +285,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     long long off = first - (upto - mine);
     int s = s_lo;
     TreeSeq q = q_lo;
-    for (long long n; off >= (n = blocks_of(q)); q = tree_seq(p, ++s)) off -= n;
-    const int unit = static_cast<int>(tree_div(off, q.blocks));
-    start[0] = s, start[1] = unit / q.pairs, start[2] = unit % q.pairs;
-    start[3] = static_cast<int>(off - static_cast<long long>(unit) * q.blocks);
+    for (long long n; off >= (n = cost_of(q)); q = tree_seq(p, ++s)) off -= n;
+    const int hk = static_cast<int>(tree_div(off, tree_head_cost(p, q)));
+    off -= hk * tree_head_cost(p, q);
+    const int pr = static_cast<int>(min(tree_div(off, tree_pair_cost(q)), static_cast<long long>(q.pairs - 1)));
+    start[0] = s, start[1] = hk, start[2] = pr, start[3] = static_cast<int>(off - pr * tree_pair_cost(q));
     start[4] = q.tok0, start[5] = q.q_len, start[6] = q.ctx, start[7] = q.end, start[8] = q.blocks, start[9] = q.pairs;
   }
   tc_fence_before_sync();
@@ -270,7 +303,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   {
     const int word = lane < 10 ? start[lane] : 0;
     auto get = [&](int i) { return __shfl_sync(0xFFFFFFFFu, word, i); };
-    walk.s = get(0), walk.hk = get(1), walk.pr = get(2), walk.j = get(3);
+    walk.s = get(0), walk.hk = get(1), walk.pr = get(2), walk.at = get(3);
     walk.q.tok0 = get(4), walk.q.q_len = get(5), walk.q.ctx = get(6), walk.q.end = get(7), walk.q.blocks = get(8);
     walk.q.pairs = get(9), walk.left = __shfl_sync(0xFFFFFFFFu, count, 0);
   }
@@ -288,7 +321,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const bool loads = lane < 2 * boxes;
     const uint32_t lane_off = half * (L::KV_BYTES / 2) + box * box_bytes;
     auto wait = [&](uint32_t b, uint32_t parity) {
-      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, TJX_ERR_WAIT_EMPTY)) != 0;
+      return tree_wait(b, parity, abort_flag, p.status, TJX_ERR_WAIT_EMPTY);
     };
     TreePortion u;
     while (ok && walk.next(p, u)) {
@@ -344,7 +377,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const uint32_t idesc_qk = idesc_bf16_f32(128, TR_BLOCK, 0, 0);  // Q and K both K-major
     const uint32_t idesc_pv = idesc_bf16_f32(128, TR_D, 0, 1);      // P from TMEM, V MN-major
     auto wait = [&](uint32_t b, uint32_t parity, int code) {
-      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, code)) != 0;
+      return tree_wait(b, parity, abort_flag, p.status, code);
     };
     // A group's blocks of a portion: all of them, or with one row tile those of its parity, counted over the run.
     auto first_of = [&](const TreePortion& u, int before) { return u.two ? 0 : (t - before) & 1; };
@@ -421,14 +454,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     int looked = 0, looked_both = 0, joined = 0;
     bool ok = true;
     auto wait = [&](uint32_t b, uint32_t parity, int code) {
-      return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.status, code)) != 0;
+      return tree_wait(b, parity, abort_flag, p.status, code);
     };
     // The product of the group's job c is in the output. A wait tells a barrier's phase from the one before it only, and
     // the scores of job c say that job c - 2 is through, not job c - 1: so even and odd jobs have barriers of their own.
     auto output_done = [&](int c) { return wait(o_done(t, c & 1), (c >> 1) & 1, TJX_ERR_WAIT_OTHER); };
     if (threadIdx.x == 96) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-    TreePortion u;
-    while (ok && walk.next(p, u)) {
+    TreePortion u, next;
+    for (bool more = walk.next(p, next); ok && more;) {
+      u = next;
       const int n_blocks = u.j1 - u.j0;
       const int tile = u.two ? t : 0;
       const int tile_nodes = u.two ? (tile == 0 ? p.tile_nodes : u.nodes - p.tile_nodes) : u.nodes;
@@ -437,73 +471,34 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       const int node = row / p.group;           // in its tile
       const bool mine_valid = row < rows;
       const int tok = u.tok + tile * p.tile_nodes + node;
-      const int32_t* mask = p.tree_mask + static_cast<size_t>(mine_valid ? tok : 0) * p.words;
-      const int words = mine_valid ? p.words : 0;
+      TreeMask mask;
+      mask.row = p.tree_mask + static_cast<size_t>(mine_valid ? tok : 0) * p.words, mask.words = mine_valid ? p.words : 0;
+      mask.first = mask.words > 0 ? static_cast<uint32_t>(mask.row[0]) : 0u;
+      mask.second = mask.words > 1 ? static_cast<uint32_t>(mask.row[1]) : 0u;
+      const uint32_t o_tmem = tmem_base + lane_addr + 256 + t * 128;
       float m_used = TR_NOTHING, l = 0.f;
       int last_job = -1;
-      for (int block = u.two ? 0 : (t - blocks) & 1; block < n_blocks && ok; block += u.two ? 1 : 2, ++c) {
-        const int sb = c & 1, kv0 = (u.j0 + block) * TR_BLOCK;
-        const uint32_t s_tmem = tmem_base + lane_addr + t * 128 + sb * 64;
-        const uint32_t o_tmem = tmem_base + lane_addr + 256 + t * 128;
-        const bool special = kv0 + TR_BLOCK > min(u.ctx, u.end);  // positions some row does not see, or that are none
-        uint32_t bad[4] = {0, 0, 0, 0};
-        const int stage = (blocks + block) % TR_V_STAGES;
-        if (special) {
-          // What a row does not see must not reach it: zero times NaN is NaN. Rows of V past the end are zeroed, and
-          // rows holding anything but finite numbers too, which are then added by hand to the rows that see them.
-          ok = wait(v_full(stage), ((blocks + block) / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
-          if (!ok) break;
-          const int g_row = row >> 1, limit = u.end - kv0;
-          uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
-                                                g_row * 128);
-          bool odd = false;
-          if (g_row < limit) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint4 x = src[i];
-              odd |= not_finite_bf16x2(x.x) || not_finite_bf16x2(x.y) || not_finite_bf16x2(x.z) || not_finite_bf16x2(x.w);
-            }
-          }
-          uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
-          votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
-          volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
-          if (lane == 0) {
-            flags[quarter] = votes;
-            mbar_arrive(u.two ? v_seen_both : v_seen(t));
-          }
-          ok = u.two ? wait(v_seen_both, looked_both & 1, TJX_ERR_WAIT_OTHER) : wait(v_seen(t), looked & 1, TJX_ERR_WAIT_OTHER);
-          if (u.two) ++looked_both; else ++looked;
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bad[i] = flags[i];
-          if (g_row >= limit || ((flags[g_row >> 4] >> (2 * (g_row & 15))) & 1)) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) src[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        ok = wait(s_full(t, sb), (c >> 1) & 1, TJX_ERR_WAIT_TMEM_FULL);
-        if (!ok) break;
+      // Job c: its scores out of TMEM, its weights into it over them. `see0`, `see1`: the positions this row sees, where
+      // `masked`. A score that is NaN or infinite makes the row NaN, as the formula does: through the maximum, since not
+      // every way to an exponential keeps a NaN.
+      auto job = [&](auto masked, int block, uint32_t see0, uint32_t see1, uint32_t (&pk)[32]) {
+        ok = wait(s_full(t, c & 1), (c >> 1) & 1, TJX_ERR_WAIT_TMEM_FULL);
+        if (!ok) return;
         tc_fence_after_sync();
         // The scores are there, so the block's keys have been read. (An arrival here is cheaper than the issuer's commit.)
         if (quarter == 0 && lane == 0) mbar_arrive(k_empty((blocks + block) % TR_K_STAGES));
-        uint32_t pk[32];
-        uint32_t see[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         if (active) {
+          const uint32_t s_tmem = tmem_base + lane_addr + t * 128 + (c & 1) * 64;
           uint32_t v[2][32];
           tmem_ld32(s_tmem, v[0]);
           tmem_ld32(s_tmem + 32, v[1]);
-          if (special) {
-            see[0] = tree_bits(mask, words, kv0, u.ctx, u.end);
-            see[1] = tree_bits(mask, words, kv0 + 32, u.ctx, u.end);
-          }
           tmem_wait_ld();
-          if (special) {
+          if (masked.value) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((see[h] >> i) & 1)) v[h][i] = __float_as_uint(-INFINITY);
+            for (int i = 0; i < 32; ++i) {
+              if (!((see0 >> i) & 1)) v[0][i] = __float_as_uint(-INFINITY);
+              if (!((see1 >> i) & 1)) v[1][i] = __float_as_uint(-INFINITY);
+            }
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -511,60 +506,100 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 2)
               mx[(i >> 1) & 3] = fmax3_nan(mx[(i >> 1) & 3], __uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1]));
-          // A score that is NaN or infinite makes the row NaN, as the formula does: through the maximum, since not every
-          // way to an exponential keeps a NaN.
           float m_blk = fmax_nan(fmax3_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2e;
           if (m_blk == INFINITY) m_blk = NAN;
           if (last_job < 0) {
             m_used = fmax_nan(m_blk, TR_NOTHING);
-          } else if (__any_sync(0xFFFFFFFFu, !(m_blk <= m_used + TR_RESCALE))) {
+          } else if (__builtin_expect(__any_sync(0xFFFFFFFFu, !(m_blk <= m_used + TR_RESCALE)), 0)) {
             const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
             ok = output_done(c - 1);
-            if (!ok) break;
+            if (!ok) return;
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-              uint32_t o[32];
-              tmem_ld32(o_tmem + i * 32, o);
+            for (int i = 0; i < 8; ++i) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + i * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-              tmem_st32(o_tmem + i * 32, o);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+              tmem_st16(o_tmem + i * 16, o);
             }
             tmem_wait_st();
           }
-          // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention);
-          // the sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA
-          // pipe, but where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0).
+          // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention); the
+          // sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA pipe, but
+          // where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0).
           const float2 scale = make_float2(p.scale_log2e, p.scale_log2e), neg_m = make_float2(-m_used, -m_used);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto weights = [&](auto poly) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1])), scale, neg_m);
-                const float2 e = exp2_pair(x, poly.value && (i & 6) == 6);
-                sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], e);
-                pk[h * 16 + (i >> 1)] = pack_bf16(e.x, e.y);
-              }
-          };
-          if (special)
-            weights(std::false_type{});
-          else
-            weights(std::true_type{});
+            for (int i = 0; i < 32; i += 2) {
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1])), scale, neg_m);
+              const float2 e = exp2_pair(x, !masked.value && (i & 6) == 6);
+              sum[(i >> 1) & 1] = __fadd2_rn(sum[(i >> 1) & 1], e);
+              pk[h * 16 + (i >> 1)] = pack_bf16(e.x, e.y);
+            }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_st32(s_tmem, pk);
           tmem_wait_st();
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready(t, sb));
+        if (lane == 0) mbar_arrive(p_ready(t, c & 1));
         last_job = c;
-        if (active && (bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
-          // The rows of V that were taken out: added to the rows that see them, once this block's product is in.
+      };
+      int block = u.two ? 0 : (t - blocks) & 1;
+      const int step = u.two ? 1 : 2;
+      // Blocks that every row sees whole.
+      const int plain = min(max(min(u.ctx, u.end) / TR_BLOCK - u.j0, 0), n_blocks);
+      for (; block < plain && ok; block += step, ++c) {
+        uint32_t pk[32];
+        job(std::false_type{}, block, 0u, 0u, pk);
+      }
+      // Blocks with positions that some row does not see, or that are none. What a row does not see must not reach it: zero
+      // times NaN is NaN. So rows of V past the end are zeroed, and rows holding anything but finite numbers too, which are
+      // then added by hand to the rows that see them.
+      for (; block < n_blocks && ok; block += step, ++c) {
+        const int kv0 = (u.j0 + block) * TR_BLOCK, stage = (blocks + block) % TR_V_STAGES;
+        ok = wait(v_full(stage), ((blocks + block) / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
+        if (!ok) break;
+        const int v_row = row >> 1, limit = u.end - kv0;
+        uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
+                                              v_row * 128);
+        bool odd = false;
+        if (v_row < limit && v_row >= u.ctx - kv0) {  // (what lies before the nodes every row sees)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint4 x = src[(i + v_row) & 7];  // (eight rows at a time, each at another bank)
+            odd |= not_finite_bf16x2(x.x) || not_finite_bf16x2(x.y) || not_finite_bf16x2(x.z) || not_finite_bf16x2(x.w);
+          }
+        }
+        uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
+        votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
+        volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
+        if (lane == 0) {
+          flags[quarter] = votes;
+          mbar_arrive(u.two ? v_seen_both : v_seen(t));
+        }
+        ok = u.two ? wait(v_seen_both, looked_both & 1, TJX_ERR_WAIT_OTHER) : wait(v_seen(t), looked & 1, TJX_ERR_WAIT_OTHER);
+        if (u.two) ++looked_both; else ++looked;
+        if (!ok) break;
+        uint32_t bad[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad[i] = flags[i];
+        if (v_row >= limit || ((flags[v_row >> 4] >> (2 * (v_row & 15))) & 1)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) src[(i + v_row) & 7] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        const uint32_t see0 = tree_bits(mask, kv0, u.ctx, u.end), see1 = tree_bits(mask, kv0 + 32, u.ctx, u.end);
+        uint32_t pk[32];
+        job(std::true_type{}, block, see0, see1, pk);
+        if (ok && active && (bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
+          // The rows of V that were taken out, once this block's product is in.
           ok = output_done(c);
           if (!ok) break;
           tc_fence_after_sync();
@@ -575,7 +610,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           for (int g = 0; g < TR_BLOCK; ++g) {
             const uint32_t some = g < 32 ? (g < 16 ? bad[0] : bad[1]) : (g < 48 ? bad[2] : bad[3]);
             if (!((some >> (2 * (g & 15))) & 1)) continue;
-            const bool sees = ((g < 32 ? see[0] : see[1]) >> (g & 31)) & 1;
+            const bool sees = ((g < 32 ? see0 : see1) >> (g & 31)) & 1;
             const uint32_t pair = weights_of[g >> 1];
             const float weight = (g & 1) ? bf16_hi(pair) : bf16_lo(pair);
             const int pos = kv0 + g;  // (below the end)
@@ -583,19 +618,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             const uint32_t* vrow = reinterpret_cast<const uint32_t*>(
                 p.kv_cache + (((static_cast<size_t>(page) * p.page_size + pos % p.page_size) * p.Hkv + u.hk) * 2 + 1) * TR_D);
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-              uint32_t o[32];
-              tmem_ld32(o_tmem + i * 32, o);
+            for (int i = 0; i < 8; ++i) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + i * 16, o);
               tmem_wait_ld();
               if (sees) {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                  const uint32_t w = vrow[i * 16 + x];
+                for (int x = 0; x < 8; ++x) {
+                  const uint32_t w = vrow[i * 8 + x];
                   o[2 * x] = __float_as_uint(fmaf(weight, bf16_lo(w), __uint_as_float(o[2 * x])));
                   o[2 * x + 1] = __float_as_uint(fmaf(weight, bf16_hi(w), __uint_as_float(o[2 * x + 1])));
                 }
               }
-              tmem_st32(o_tmem + i * 32, o);
+              tmem_st16(o_tmem + i * 16, o);
               tmem_wait_st();
             }
           }
@@ -603,6 +638,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
       }
       if (!ok) break;
+      more = walk.next(p, next);  // (while the last products run)
       // The portion's end: normalised rows, or a partial result for the join.
       if (last_job >= 0) ok = output_done(last_job);
       if (!ok) break;
@@ -687,18 +723,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           }
 #pragma unroll 1
           for (int i = 2 * t; i < 2 * t + 2; ++i) {
+            uint32_t o0[32], o1[32];
+            tmem_ld32(tmem_base + lane_addr + 256 + i * 32, o0);
+            tmem_ld32(tmem_base + lane_addr + 384 + i * 32, o1);
+            tmem_wait_ld();
             float f[32];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) f[x] = 0.f;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              if (!has[g]) continue;
-              uint32_t o[32];
-              tmem_ld32(tmem_base + lane_addr + 256 + g * 128 + i * 32, o);
-              tmem_wait_ld();
-              const float w = g == 0 ? w0 : w1;
-#pragma unroll
-              for (int x = 0; x < 32; ++x) f[x] = fmaf(__uint_as_float(o[x]), w, f[x]);
+            for (int x = 0; x < 32; ++x) {  // (a group without a block has left nothing to read: selected, not weighed)
+              f[x] = has[0] ? __uint_as_float(o0[x]) * w0 : 0.f;
+              f[x] = has[1] ? fmaf(__uint_as_float(o1[x]), w1, f[x]) : f[x];
             }
             store32(i * 32, f);
           }
@@ -712,7 +745,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         tc_fence_after_sync();
       }
       if (u.starts && !u.whole && threadIdx.x == 96)
-        p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + (u.after + share - 1) / share));
+        p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + 1 + tree_div(u.past, share)));
       blocks += n_blocks;
     }
   }
