@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import struct
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -685,52 +686,60 @@ def rpa_plan(ctx_lens: torch.Tensor, q_lens: torch.Tensor, page_indices: torch.T
     plus its depth, while its slot stays that of its index. `out` is written instead of new tensors; it may not overlap
     the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into ctx_lens)."""
     inputs = [ctx_lens, q_lens, page_indices, free_pages, n_free]
-    for name, t in zip(("ctx_lens", "q_lens", "page_indices", "free_pages", "n_free"), inputs):
-        if t.dtype is not torch.int32 or t.dim() != 1:
+    shapes = [t.shape for t in inputs]
+    for name, t, shape in zip(("ctx_lens", "q_lens", "page_indices", "free_pages", "n_free"), inputs, shapes):
+        if t.dtype is not torch.int32 or len(shape) != 1:
             raise ValueError(f"{name} must be an int32 vector")
-    S, T, entries = ctx_lens.shape[0], int(tokens), page_indices.shape[0]
-    if S == 0 or q_lens.shape[0] != S or entries == 0 or entries % S:
+    (S,), (S_new,), (entries,), (capacity,), (counts,) = shapes
+    T = int(tokens)
+    if S == 0 or S_new != S or entries == 0 or entries % S:
         raise ValueError("ctx_lens and q_lens are (S,), page_indices (S * pages_per_seq,)")
-    if n_free.shape[0] < 1:
+    if counts < 1:
         raise ValueError("n_free holds the number of free pages")
+    held_ptr = depths_ptr = None
     if pages_held is not None:
         inputs.append(pages_held)
+        held_ptr = pages_held.data_ptr()
         if pages_held.shape != (S,) or pages_held.dtype is not torch.int32:
             raise ValueError("pages_held is int32 (S,)")
     if depths is not None:
         inputs.append(depths)
+        depths_ptr = depths.data_ptr()
         if depths.shape != (T,) or depths.dtype is not torch.int32:
             raise ValueError("depths is int32 (tokens,)")
     if T < 0 or page_size <= 0:
         raise ValueError("page_size must be positive and tokens not negative")
     device = _need_cuda(*inputs)
     if out is None:
-        out = RpaStep(*torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device)
-                      .split_with_sizes((S, S + 1, T, T, S, 2)))
+        block = torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device)
+        out = RpaStep._make(block.split_with_sizes((S, S + 1, T, T, S, 2)))
+        at = block.data_ptr()
+        outputs = (at, at + 4 * S, at + 8 * S + 4, at + 8 * S + 4 + 4 * T, at + 8 * S + 4 + 8 * T, at + 12 * S + 4 + 8 * T)
     else:
         _need_cuda(ctx_lens, *out)
         if [tuple(t.shape) for t in out] != [(S,), (S + 1,), (T,), (T,), (S,), (2,)] or any(t.dtype is not torch.int32 for t in out):
             raise ValueError("out is a step of other sizes")
         if any(_overlap(a, b) for a in out for b in inputs):
             raise ValueError("out overlaps an input")
-    _launch(device, "tjx_rpa_plan", ctx_lens.data_ptr(), q_lens.data_ptr(), None if pages_held is None else pages_held.data_ptr(),
-            None if depths is None else depths.data_ptr(), page_indices.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(),
-            free_pages.shape[0], S, T, entries // S, page_size, *[t.data_ptr() for t in out])
+        outputs = [t.data_ptr() for t in out]
+    _launch(device, "tjx_rpa_plan", ctx_lens.data_ptr(), q_lens.data_ptr(), held_ptr, depths_ptr, page_indices.data_ptr(),
+            free_pages.data_ptr(), n_free.data_ptr(), capacity, S, T, entries // S, page_size, *outputs)
     return out
 
 
-_NormRopeStrides = ctypes.c_int64 * 10
+_pack_strides = struct.Struct("10q").pack
 
 
-def _heads(name: str, t: torch.Tensor, tokens: int, D: int) -> tuple[int, int, int]:
-    """Heads, token stride and head stride of a (tokens, heads, D) operand."""
+def _heads(name: str, t: torch.Tensor, tokens: int, D: int) -> tuple[int, int, int, int]:
+    """Heads, token stride, head stride and address of a (tokens, heads, D) operand."""
     shape = t.shape
     if len(shape) != 3 or t.dtype is not torch.bfloat16 or shape[0] != tokens or shape[2] != D:
         raise ValueError(f"{name} must be bfloat16 ({tokens}, heads, {D})")
     token, head, dense = t.stride()
-    if dense != 1 or token % 4 or head % 4 or t.data_ptr() % 8:
+    at = t.data_ptr()
+    if dense != 1 or (token | head) & 3 or at & 7:
         raise ValueError(f"{name}'s last dimension must be dense, its strides multiples of 4 elements, its data 8-byte aligned")
-    return shape[1], token, head
+    return shape[1], token, head, at
 
 
 def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -738,67 +747,65 @@ def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, kv_cache, slots, eps, interleaved):
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("q is (T, H, D)")
-    T, H, D = q.shape
-    _, q_tok, q_head = _heads("q", q, T, D)
-    Hkv, k_tok, k_head = _heads("k", k, T, D)
-    if (q_gamma is None) != (k_gamma is None):
-        raise ValueError("q_gamma and k_gamma are given together or not at all")
+    T, H, D = shape
+    _, q_tok, q_head, q_at = _heads("q", q, T, D)
+    Hkv, k_tok, k_head, k_at = _heads("k", k, T, D)
+    v_tok = v_head = n_slots = ko_tok = ko_head = 0
+    v_at = qg_at = kg_at = slots_at = ko_at = cache_at = None
     dense = [positions, cos_sin]
-    if q_gamma is not None:
+    if q_gamma is not None and k_gamma is not None:
         dense += (q_gamma, k_gamma)
-        for g in (q_gamma, k_gamma):
-            if g.shape != (D,) or g.dtype is not torch.bfloat16 or g.data_ptr() % 8:
-                raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
+        qg_at, kg_at = q_gamma.data_ptr(), k_gamma.data_ptr()
+        if q_gamma.shape != (D,) or k_gamma.shape != (D,) or q_gamma.dtype is not torch.bfloat16 \
+                or k_gamma.dtype is not torch.bfloat16 or (qg_at | kg_at) & 7:
+            raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
+    elif q_gamma is not k_gamma:
+        raise ValueError("q_gamma and k_gamma are given together or not at all")
     if positions.shape != (T,) or positions.dtype is not torch.int32:
         raise ValueError("positions is int32 (T,)")
-    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32 or cos_sin.shape[1] > D or cos_sin.shape[1] % 8 \
-            or cos_sin.shape[0] == 0 or cos_sin.data_ptr() % 16:
+    table, table_at = cos_sin.shape, cos_sin.data_ptr()
+    if len(table) != 2 or cos_sin.dtype is not torch.float32 or table[1] > D or table[1] & 7 or table[0] == 0 or table_at & 15:
         raise ValueError("cos_sin is float32 (max_positions, rot), rot a multiple of 8 up to the head dimension, 16-byte aligned")
-    used = (q, k)
-    v_tok = v_head = slots_ptr = n_slots = 0
+    used = [q, k]
     if kv_cache is not None:
-        used = (q, k, v)
-        _, v_tok, v_head = _heads("v", v, T, D)
+        used.append(v)
+        _, v_tok, v_head, v_at = _heads("v", v, T, D)
         dense += (slots, kv_cache)
-        slots_ptr, n_slots = slots.data_ptr(), kv_cache.shape[0] * kv_cache.shape[1]
+        slots_at, cache_at, n_slots = slots.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0] * kv_cache.shape[1]
     device = _need_cuda(*dense)
+    index = device.index
     for t in used:
-        if t.get_device() != device.index:
+        if t.get_device() != index:
             raise ValueError("all tensors must be on the same device")
     if q_out is None:
-        q_out = torch.empty((T, H, D), dtype=torch.bfloat16, device=device)
-        qo_tok, qo_head = H * D, D
+        q_out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        qo_tok, qo_head, qo_at = H * D, D, q_out.data_ptr()
     else:
-        heads, qo_tok, qo_head = _heads("the queries' output", q_out, T, D)
+        heads, qo_tok, qo_head, qo_at = _heads("the queries' output", q_out, T, D)
         if heads != H or q_out.device != device or any(_overlap(q_out, t) for t in used if not _same(q_out, q)):
             raise ValueError("the queries' output is q itself or memory of its own, like q")
-    ko_tok = ko_head = 0
-    if kv_cache is None:
-        if k_out is None:
-            k_out = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
-            ko_tok, ko_head = Hkv * D, D
-        else:
-            heads, ko_tok, ko_head = _heads("the keys' output", k_out, T, D)
-            if heads != Hkv or k_out.device != device \
-                    or any(_overlap(k_out, t) for t in (q, k, q_out) if not _same(k_out, k)):
-                raise ValueError("the keys' output is k itself or memory of its own, like k")
-    else:
-        lo = kv_cache.data_ptr()
-        hi = lo + 2 * kv_cache.numel()
-        for at, heads, token, head in ((q.data_ptr(), H, q_tok, q_head), (k.data_ptr(), Hkv, k_tok, k_head),
-                                       (v.data_ptr(), Hkv, v_tok, v_head), (q_out.data_ptr(), H, qo_tok, qo_head)):
-            if at < hi and at + 2 * ((T - 1) * token + (heads - 1) * head + D) > lo:
+    if kv_cache is not None:
+        behind = cache_at + 2 * n_slots * 2 * Hkv * D
+        for at, heads, token, head in ((q_at, H, q_tok, q_head), (k_at, Hkv, k_tok, k_head), (v_at, Hkv, v_tok, v_head),
+                                       (qo_at, H, qo_tok, qo_head)):
+            if at < behind and at + 2 * ((T - 1) * token + (heads - 1) * head + D) > cache_at:
                 raise ValueError("the cache overlaps an operand")
+    elif k_out is None:
+        k_out = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
+        ko_tok, ko_head, ko_at = Hkv * D, D, k_out.data_ptr()
+    else:
+        heads, ko_tok, ko_head, ko_at = _heads("the keys' output", k_out, T, D)
+        if heads != Hkv or k_out.device != device or any(_overlap(k_out, t) for t in (q, k, q_out) if not _same(k_out, k)):
+            raise ValueError("the keys' output is k itself or memory of its own, like k")
     if T == 0:
         return q_out, k_out
-    strides = _NormRopeStrides(q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head)
-    _launch(device, "tjx_norm_rope_bf16", q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), strides,
-            None if q_gamma is None else q_gamma.data_ptr(), None if k_gamma is None else k_gamma.data_ptr(),
-            positions.data_ptr(), cos_sin.data_ptr(), slots_ptr or None, q_out.data_ptr(),
-            None if k_out is None else k_out.data_ptr(), None if kv_cache is None else kv_cache.data_ptr(), T, H, Hkv, D,
-            cos_sin.shape[1], cos_sin.shape[0], 1 if interleaved else 0, n_slots, eps)
+    _launch(device, "tjx_norm_rope_bf16", q_at, k_at, v_at,
+            _pack_strides(q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head), qg_at, kg_at,
+            positions.data_ptr(), table_at, slots_at, qo_at, ko_at, cache_at, T, H, Hkv, D, table[1], table[0],
+            1 if interleaved else 0, n_slots, eps)
     return q_out, k_out
 
 
@@ -822,13 +829,14 @@ def rpa_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gam
     """`qk_norm_rope` with the cache write in the same pass: the turned key and the value of token t go to row slots[t]
     (page * page_size + row, as `rpa_plan` gives it; out of range: not written; no slot twice) of the cache
     (pages, page_size, Hkv, 2, D), IN PLACE. Returns (q', the cache); `out=q` updates the queries in place."""
-    if kv_cache.dim() != 5 or kv_cache.shape[3] != 2 or kv_cache.dtype is not torch.bfloat16 or kv_cache.numel() == 0:
+    cache, q_shape, k_shape = kv_cache.shape, q.shape, k.shape
+    if len(cache) != 5 or cache[3] != 2 or kv_cache.dtype is not torch.bfloat16 or 0 in cache:
         raise ValueError("the cache is (pages, page_size, Hkv, 2, D) bfloat16: each head's key and value side by side")
-    if q.dim() != 3 or k.shape != v.shape or k.shape[1:] != (kv_cache.shape[2], kv_cache.shape[4]):
+    if len(q_shape) != 3 or k_shape != (q_shape[0], cache[2], cache[4]) or v.shape != k_shape:
         raise ValueError("q is (T, H, D), k and v (T, Hkv, D) with the cache's Hkv and D")
-    if kv_cache.shape[0] * kv_cache.shape[1] >= 1 << 31:
+    if cache[0] * cache[1] >= 1 << 31:
         raise ValueError("the cache's rows must fit in int32")
-    if slots.shape != (q.shape[0],) or slots.dtype is not torch.int32:
+    if slots.shape != (q_shape[0],) or slots.dtype is not torch.int32:
         raise ValueError("slots is int32 (T,)")
     q_out, _ = _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, out, None, kv_cache, slots, eps, interleaved)
     return q_out, kv_cache
