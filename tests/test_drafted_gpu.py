@@ -107,6 +107,7 @@ def close(got, want, size, slack=2.0**-20):
     (2, 1, 1, 256, 8, True, True),
     (700, 7, 3, 64, 32, True, False),
     (4, 4, 4, 128, 0, False, True),        # the norm alone
+    (6, 5, 2, 128, 24, False, True),       # a rotated part that is not two halves of whole lanes
 ])
 def test_norm_and_rotation(T, H, Hkv, D, rot, interleaved, norm):
     rng = np.random.default_rng(T)
@@ -144,6 +145,34 @@ def test_norm_and_rotation(T, H, Hkv, D, rot, interleaved, norm):
     ops.qk_norm_rope(dq, dk, *args, eps=1e-5, interleaved=interleaved, out=(dq, dk))
     assert torch.equal(dq, got[0]) and torch.equal(dk, got[1])
     np.testing.assert_array_equal(to_host(dv).view(np.uint16), v.view(np.uint16))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_and_rotation_of_rows_eight_bytes_apart_from_sixteen(interleaved):
+    # Token and head strides that are multiples of 4 elements but not of 8, and a base in between.
+    rng = np.random.default_rng(3)
+    T, H, Hkv, D = 9, 6, 2, 128
+    table, gammas = angles(64, 64), [rand_bf16((D,), i) for i in (1, 2)]
+    positions = rng.integers(0, 64, T).astype(np.int32)
+    wide = rand_bf16((T, H + Hkv, D + 12), 4)
+    q, k = wide[:, :H, 4 : 4 + D], wide[:, H:, 4 : 4 + D]
+    want = [oracle.norm_rope_f64(x, g, positions, table, 1e-6, interleaved) for x, g in zip((q, k), gammas)]
+    dev = to_device(wide)
+    got = ops.qk_norm_rope(dev[:, :H, 4 : 4 + D], dev[:, H:, 4 : 4 + D], *map(to_device, gammas), to_device(positions),
+                           to_device(table), interleaved=interleaved)
+    for g, (w, size) in zip(got, want):
+        close(to_host(g), w, size)
+
+
+def test_an_infinity_stays_where_it_is():
+    # Without the norm an infinite element turns its pair and nothing else; elements past the rotated part stay as they are.
+    for rot, interleaved in ((64, False), (64, True), (24, False)):
+        x = rand_bf16((2, 1, 128), 5)
+        x[0, 0, 100] = np.inf
+        got = to_host(ops.qk_norm_rope(to_device(x), to_device(x), None, None, dev32([3, 4]), to_device(angles(8, rot)),
+                                       interleaved=interleaved)[0])
+        assert np.isinf(f64(got[0, 0, 100])) and np.isfinite(np.delete(f64(got[0, 0]), 100)).all()
+        np.testing.assert_array_equal(got[..., rot:].view(np.uint16), x[..., rot:].view(np.uint16))
 
 
 def test_norm_and_rotation_refuse_overlapping_outputs_and_unknown_heads():

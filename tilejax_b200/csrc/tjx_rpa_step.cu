@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) rpa_plan_kernel(const PlanParams
 
 constexpr int NR_THREADS = 256;
 constexpr int NR_UNROLL = 4;
+constexpr int NR_BLOCKS = 2;  // CTAs of an SM. Fewer or more of them, or of rows in flight, are slower: 4096 tokens of 32 + 8
+                              // + 8 heads 21.5 us; 30 with one CTA, 29 with three; 24 with two, five or six rows a lane
 
 struct NormRopeParams {
   const __nv_bfloat16 *q, *k, *v;                // v: or null (no cache)
@@ -175,103 +177,167 @@ struct NormRopeParams {
   long long q_head, k_head, v_head, qo_head, ko_head;  // ... and from one head to the next
   const int32_t *positions, *slots;
   const float* cos_sin;  // [max_positions, rot]: cosines, then sines
-  int T, H, Hkv, rot, max_positions, interleaved, n_slots;
+  int T, H, Hkv, rot, max_positions, n_slots;
+  bool wide;  // every row starts at a multiple of 16 bytes (else of 8)
   float eps;
 };
 
-// A lane holds eight elements of a head's row in two runs of four, at a and b: the two halves of four rotated pairs
-// (half-split: pair i is elements i and i + rot / 2) or four neighbouring pairs (interleaved), either way the pairs
-// 4 u .. 4 u + 3 of lane u; lanes past the rotated part hold eight elements that are only normed. So the rotation
-// needs no exchange between lanes, and each lane reads four cosines and four sines once for all heads of its token.
-// D / 8 lanes make a row, and a warp keeps NR_UNROLL rows a lane in flight. Everything is f32 from the load to the one
-// rounding of the result. Bound by HBM: each row is read once and written once.
-template <int D>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const NormRopeParams p) {
+// D / 8 lanes make a row; a lane holds eight elements of it as four pairs that rotate together: 4 u .. 4 u + 3 of lane u,
+// which are 16 neighbouring bytes where pairs are neighbours (NEIGHBOURS), else two runs of four, one in each half of the
+// rotated part; lanes past it hold elements that are only normed. So the rotation needs no exchange between lanes. With
+// (a, b) a pair, g its gammas and r = 1 / rms:  r (a g_a cos - b g_b sin),  r (a g_a sin + b g_b cos), the four products of
+// gamma and angle made once for all heads of the token, everything f32 from the load to the one rounding of the result.
+//
+// Heads come in chunks of one kind (queries, keys, values), NR_UNROLL rows a lane. The chunks of all tokens, in order, are
+// cut into equal runs, one for each warp the GPU holds at a time (a single token's chunks each get a warp), and a warp has
+// the next chunk's rows, and the next token's angles, on their way while it works on one. Each row is read once and written
+// once; beside the memory the issue of instructions bounds it: 130 for two rows of 128 (issue slots 60 % busy) where
+// unfolded factors, one element an instruction and shuffles between the halves took 200 (77 %). 4096 tokens of 32 + 8 + 8
+// heads 21.5 us (4.8 TB/s), 16384 of 32 + 8 without a cache 62.5 us (5.4 TB/s).
+template <int D, bool NEIGHBOURS>
+__global__ void __launch_bounds__(NR_THREADS, NR_BLOCKS) norm_rope_kernel(const NormRopeParams p) {
   constexpr int LANES = D / 8;            // lanes per row
   constexpr int PER_PASS = 32 / LANES;    // rows per warp and pass
   constexpr int ROWS = PER_PASS * NR_UNROLL;
   const int lane = threadIdx.x & 31, u = lane % LANES, sub = lane / LANES;
-  const int heads = p.H + p.Hkv + (p.v != nullptr ? p.Hkv : 0);
-  const int chunks = (heads + ROWS - 1) / ROWS;
-  const long long items = static_cast<long long>(p.T) * chunks;
+  const int chunks_q = (p.H + ROWS - 1) / ROWS, chunks_k = (p.Hkv + ROWS - 1) / ROWS;
+  const int chunks = chunks_q + (p.v != nullptr ? 2 : 1) * chunks_k;
+  const long long total = static_cast<long long>(p.T) * chunks, warps = static_cast<long long>(gridDim.x) * (NR_THREADS / 32);
+  const long long warp = static_cast<long long>(blockIdx.x) * (NR_THREADS / 32) + (threadIdx.x >> 5);
+  const long long run = warp * total / warps, run_end = (warp + 1) * total / warps;
+  if (run >= run_end) return;
+  int tok = static_cast<int>(run / chunks), chunk = static_cast<int>(run % chunks);
   const bool rotated = u < p.rot / 8;
-  const int a = rotated ? (p.interleaved ? 8 * u : 4 * u) : p.rot + 8 * (u - p.rot / 8);
-  const int b = rotated && !p.interleaved ? p.rot / 2 + 4 * u : a + 4;
-  const int warps = gridDim.x * (NR_THREADS / 32);
-  for (long long item = blockIdx.x * (NR_THREADS / 32) + (threadIdx.x >> 5); item < items; item += warps) {
-    const int tok = static_cast<int>(item / chunks), row0 = static_cast<int>(item % chunks) * ROWS + sub;
-    uint2 xa[NR_UNROLL], xb[NR_UNROLL];
+  // The lane's elements: a .. a + 3 and b .. b + 3.
+  const int a = !NEIGHBOURS && rotated ? 4 * u : 8 * u;
+  const int b = !NEIGHBOURS && rotated ? p.rot / 2 + 4 * u : a + 4;
+  const bool wide = NEIGHBOURS && p.wide;
+  auto load = [&](const __nv_bfloat16* src) {
+    if (wide) return *reinterpret_cast<const uint4*>(src + a);
+    const uint2 lo = *reinterpret_cast<const uint2*>(src + a), hi = *reinterpret_cast<const uint2*>(src + b);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+  // Kind of a chunk (0 queries, 1 keys, 2 values) and its first head.
+  auto kind_of = [&](int chunk) { return chunk < chunks_q ? 0 : chunk < chunks_q + chunks_k ? 1 : 2; };
+  auto head_of = [&](int chunk, int kind) { return (chunk - (kind == 0 ? 0 : kind == 1 ? chunks_q : chunks_q + chunks_k)) * ROWS; };
+  auto load_chunk = [&](int tok, int chunk, uint4 (&x)[NR_UNROLL]) {
+    const int kind = kind_of(chunk), r0 = head_of(chunk, kind) + sub;
+    const __nv_bfloat16* src = kind == 0 ? p.q + tok * p.q_tok : kind == 1 ? p.k + tok * p.k_tok : p.v + tok * p.v_tok;
+    const long long head = kind == 0 ? p.q_head : kind == 1 ? p.k_head : p.v_head;
+    const int heads = kind == 0 ? p.H : p.Hkv;
 #pragma unroll
     for (int i = 0; i < NR_UNROLL; ++i) {
-      const int r = row0 + i * PER_PASS;
-      const __nv_bfloat16* src = nullptr;
-      if (r < p.H) src = p.q + tok * p.q_tok + r * p.q_head;
-      else if (r < p.H + p.Hkv) src = p.k + tok * p.k_tok + (r - p.H) * p.k_head;
-      else if (r < heads) src = p.v + tok * p.v_tok + (r - p.H - p.Hkv) * p.v_head;
-      xa[i] = xb[i] = make_uint2(0, 0);
-      if (src != nullptr) {
-        xa[i] = *reinterpret_cast<const uint2*>(src + a);
-        xb[i] = *reinterpret_cast<const uint2*>(src + b);
+      const int r = r0 + i * PER_PASS;
+      x[i] = r < heads ? load(src + r * head) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  // Pairs j = 2 h and 2 h + 1 of a lane's words, first and second elements.
+  auto unpack = [](const uint4& w, float2 (&fa)[2], float2 (&fb)[2]) {
+    if (NEIGHBOURS) {
+      fa[0] = make_float2(bf16_lo(w.x), bf16_lo(w.y)), fb[0] = make_float2(bf16_hi(w.x), bf16_hi(w.y));
+      fa[1] = make_float2(bf16_lo(w.z), bf16_lo(w.w)), fb[1] = make_float2(bf16_hi(w.z), bf16_hi(w.w));
+    } else {
+      fa[0] = make_float2(bf16_lo(w.x), bf16_hi(w.x)), fa[1] = make_float2(bf16_lo(w.y), bf16_hi(w.y));
+      fb[0] = make_float2(bf16_lo(w.z), bf16_hi(w.z)), fb[1] = make_float2(bf16_lo(w.w), bf16_hi(w.w));
+    }
+  };
+  // A token's angles: of its position, clamped to the table as a gather's index is.
+  auto load_angles = [&](int position, float4& cs, float4& sn) {
+    cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!rotated) return;
+    const float* table = p.cos_sin + static_cast<size_t>(min(max(position, 0), p.max_positions - 1)) * p.rot + 4 * u;
+    cs = *reinterpret_cast<const float4*>(table), sn = *reinterpret_cast<const float4*>(table + p.rot / 2);
+  };
+  uint4 x[NR_UNROLL];
+  load_chunk(tok, chunk, x);
+  float4 cs, sn;
+  load_angles(p.positions[tok], cs, sn);
+  int slot = p.slots != nullptr ? p.slots[tok] : -1;
+  int position_ahead = tok + 1 < p.T ? p.positions[tok + 1] : 0;
+  int slot_ahead = p.slots != nullptr && tok + 1 < p.T ? p.slots[tok + 1] : -1;
+  int have = -1;  // the kind the factors are of
+  float2 aa[2], ab[2], ba[2], bb[2];  // first = a aa + b ab, second = a ba + b bb
+  for (long long at = run; at < run_end; ++at) {
+    uint4 ahead[NR_UNROLL];
+    float4 cs_ahead = cs, sn_ahead = sn;
+    const bool new_token = chunk + 1 == chunks;
+    if (at + 1 < run_end) {
+      load_chunk(new_token ? tok + 1 : tok, new_token ? 0 : chunk + 1, ahead);
+      if (new_token) load_angles(position_ahead, cs_ahead, sn_ahead);
+    }
+    const int kind = kind_of(chunk), r0 = head_of(chunk, kind) + sub;
+    if (kind != have && kind < 2) {
+      have = kind;
+      float2 ga[2] = {make_float2(1.f, 1.f), make_float2(1.f, 1.f)}, gb[2] = {ga[0], ga[0]};
+      if (p.q_gamma != nullptr) unpack(load(kind == 0 ? p.q_gamma : p.k_gamma), ga, gb);
+      const float2 c[2] = {make_float2(cs.x, cs.y), make_float2(cs.z, cs.w)}, s[2] = {make_float2(sn.x, sn.y), make_float2(sn.z, sn.w)};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        aa[h] = __fmul2_rn(ga[h], c[h]), bb[h] = __fmul2_rn(gb[h], c[h]), ba[h] = __fmul2_rn(ga[h], s[h]);
+        ab[h] = __fmul2_rn(gb[h], make_float2(-s[h].x, -s[h].y));
       }
     }
-    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (rotated) {
-      const int pos = min(max(p.positions[tok], 0), p.max_positions - 1);  // clamped, as a gather's index is
-      const float* table = p.cos_sin + static_cast<size_t>(pos) * p.rot;
-      c = *reinterpret_cast<const float4*>(table + 4 * u);
-      s = *reinterpret_cast<const float4*>(table + p.rot / 2 + 4 * u);
-    }
-    const int slot = p.slots != nullptr ? p.slots[tok] : -1;
+    __nv_bfloat16* dst = nullptr;
+    long long head = 0;
+    if (kind == 0)
+      dst = p.q_out + tok * p.qo_tok, head = p.qo_head;
+    else if (p.kv_cache == nullptr)
+      dst = p.k_out + tok * p.ko_tok, head = p.ko_head;
+    else if (slot >= 0 && slot < p.n_slots)
+      dst = p.kv_cache + (static_cast<size_t>(slot) * p.Hkv * 2 + (kind - 1)) * D, head = 2 * D;
+    const int heads = dst == nullptr ? 0 : kind == 0 ? p.H : p.Hkv;
 #pragma unroll
     for (int i = 0; i < NR_UNROLL; ++i) {
-      const int r = row0 + i * PER_PASS;
-      const bool is_q = r < p.H, is_k = !is_q && r < p.H + p.Hkv;
-      uint2 oa = xa[i], ob = xb[i];
-      float x[8] = {bf16_lo(oa.x), bf16_hi(oa.x), bf16_lo(oa.y), bf16_hi(oa.y),
-                    bf16_lo(ob.x), bf16_hi(ob.x), bf16_lo(ob.y), bf16_hi(ob.y)};
-      if (p.q_gamma != nullptr) {  // (the same for every lane: the shuffles are convergent)
-        float sum = 0.f;
+      uint4 y = x[i];
+      if (kind < 2) {
+        float2 fa[2], fb[2];
+        unpack(y, fa, fb);
+        float scale = 1.f;
+        if (p.q_gamma != nullptr) {
+          float2 sum = __fmul2_rn(fa[0], fa[0]);
+          sum = __ffma2_rn(fa[1], fa[1], sum), sum = __ffma2_rn(fb[0], fb[0], sum), sum = __ffma2_rn(fb[1], fb[1], sum);
+          float squares = sum.x + sum.y;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-#pragma unroll
-        for (int d = LANES / 2; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-        const float scale = rsqrtf(sum * (1.0f / D) + p.eps);
-        if (is_q || is_k) {
-          const __nv_bfloat16* g = is_q ? p.q_gamma : p.k_gamma;
-          const uint2 ga = __ldg(reinterpret_cast<const uint2*>(g + a)), gb = __ldg(reinterpret_cast<const uint2*>(g + b));
-          const float gv[8] = {bf16_lo(ga.x), bf16_hi(ga.x), bf16_lo(ga.y), bf16_hi(ga.y),
-                               bf16_lo(gb.x), bf16_hi(gb.x), bf16_lo(gb.y), bf16_hi(gb.y)};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= scale * gv[j];
+          for (int d = LANES / 2; d >= 1; d >>= 1) squares += __shfl_xor_sync(0xFFFFFFFFu, squares, d);
+          scale = rsqrtf(fmaf(squares, 1.0f / D, p.eps));
         }
-      }
-      if (is_q || is_k) {
-        if (rotated) {
-          const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+        const float2 sc = make_float2(scale, scale);
+        float2 ya[2], yb[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float xe = p.interleaved ? x[2 * j] : x[j], xf = p.interleaved ? x[2 * j + 1] : x[j + 4];
-            const float ye = xe * cv[j] - xf * sv[j], yf = xe * sv[j] + xf * cv[j];
-            if (p.interleaved) x[2 * j] = ye, x[2 * j + 1] = yf;
-            else x[j] = ye, x[j + 4] = yf;
+        for (int h = 0; h < 2; ++h) {
+          if (rotated) {
+            ya[h] = __ffma2_rn(fa[h], aa[h], __fmul2_rn(fb[h], ab[h]));
+            yb[h] = __ffma2_rn(fa[h], ba[h], __fmul2_rn(fb[h], bb[h]));
+          } else {  // (an infinity must not meet a sine of 0)
+            ya[h] = __fmul2_rn(fa[h], aa[h]), yb[h] = __fmul2_rn(fb[h], bb[h]);
           }
+          ya[h] = __fmul2_rn(ya[h], sc), yb[h] = __fmul2_rn(yb[h], sc);
         }
-        oa = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-        ob = make_uint2(pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        y = NEIGHBOURS ? make_uint4(pack_bf16(ya[0].x, yb[0].x), pack_bf16(ya[0].y, yb[0].y), pack_bf16(ya[1].x, yb[1].x),
+                                    pack_bf16(ya[1].y, yb[1].y))
+                       : make_uint4(pack_bf16(ya[0].x, ya[0].y), pack_bf16(ya[1].x, ya[1].y), pack_bf16(yb[0].x, yb[0].y),
+                                    pack_bf16(yb[1].x, yb[1].y));
       }
-      __nv_bfloat16* dst = nullptr;
-      if (is_q) {
-        dst = p.q_out + tok * p.qo_tok + r * p.qo_head;
-      } else if (r < heads) {
-        const int h = is_k ? r - p.H : r - p.H - p.Hkv;
-        if (p.kv_cache == nullptr)
-          dst = p.k_out + tok * p.ko_tok + h * p.ko_head;
-        else if (slot >= 0 && slot < p.n_slots)
-          dst = p.kv_cache + ((static_cast<size_t>(slot) * p.Hkv + h) * 2 + (is_k ? 0 : 1)) * D;
+      const int r = r0 + i * PER_PASS;
+      if (r < heads) {
+        __nv_bfloat16* to = dst + r * head;
+        if (wide) {
+          *reinterpret_cast<uint4*>(to + a) = y;
+        } else {
+          *reinterpret_cast<uint2*>(to + a) = make_uint2(y.x, y.y);
+          *reinterpret_cast<uint2*>(to + b) = make_uint2(y.z, y.w);
+        }
       }
-      if (dst != nullptr) {
-        *reinterpret_cast<uint2*>(dst + a) = oa;
-        *reinterpret_cast<uint2*>(dst + b) = ob;
+    }
+#pragma unroll
+    for (int i = 0; i < NR_UNROLL; ++i) x[i] = ahead[i];
+    ++chunk;
+    if (new_token) {
+      chunk = 0, ++tok, have = -1;
+      cs = cs_ahead, sn = sn_ahead, slot = slot_ahead;
+      if (tok + 1 < p.T) {
+        position_ahead = p.positions[tok + 1];
+        if (p.slots != nullptr) slot_ahead = p.slots[tok + 1];
       }
     }
   }
@@ -390,12 +456,17 @@ int tjx_norm_rope_bf16(const void* q, const void* k, const void* v, const int64_
   if (D != 64 && D != 128 && D != 256) return fail(TJX_E_ARG, "head dimension must be 64, 128 or 256");
   if (rot < 0 || rot > D || rot % 8 != 0) return fail(TJX_E_ARG, "the rotated part is a multiple of 8, at most the head dimension");
   if (!(eps >= 0.f)) return fail(TJX_E_ARG, "eps must not be negative");
-  const void* aligned8[] = {q, k, v, q_gamma, k_gamma, q_out, k_out, kv_cache};
-  for (const void* ptr : aligned8)
-    if (reinterpret_cast<uintptr_t>(ptr) & 7u) return fail(TJX_E_ARG, "bf16 operands must be 8-byte aligned");
+  // 16 bytes a lane where every row allows it.
+  uintptr_t bits = 0;
+  for (const void* ptr : {q, k, v, q_gamma, k_gamma, const_cast<const void*>(q_out), const_cast<const void*>(k_out), const_cast<const void*>(kv_cache)})
+    bits |= reinterpret_cast<uintptr_t>(ptr);
+  if (bits & 7u) return fail(TJX_E_ARG, "bf16 operands must be 8-byte aligned");
   if (reinterpret_cast<uintptr_t>(cos_sin) & 15u) return fail(TJX_E_ARG, "cos_sin must be 16-byte aligned");
-  for (int i = 0; i < 10; ++i)
+  for (int i = 0; i < 10; ++i) {
     if (strides[i] % 4 != 0 || strides[i] < 0) return fail(TJX_E_ARG, "strides must be multiples of 4 elements");
+    bits |= static_cast<uintptr_t>(strides[i]) * 2;
+  }
+  const bool wide = (bits & 15u) == 0;
   NormRopeParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q), p.k = static_cast<const __nv_bfloat16*>(k);
   p.v = static_cast<const __nv_bfloat16*>(v);
@@ -405,13 +476,14 @@ int tjx_norm_rope_bf16(const void* q, const void* k, const void* v, const int64_
   p.q_tok = strides[0], p.q_head = strides[1], p.k_tok = strides[2], p.k_head = strides[3], p.v_tok = strides[4];
   p.v_head = strides[5], p.qo_tok = strides[6], p.qo_head = strides[7], p.ko_tok = strides[8], p.ko_head = strides[9];
   p.positions = positions, p.slots = slots, p.cos_sin = cos_sin;
-  p.T = T, p.H = H, p.Hkv = Hkv, p.rot = rot, p.max_positions = max_positions, p.interleaved = interleaved;
+  p.T = T, p.H = H, p.Hkv = Hkv, p.rot = rot, p.max_positions = max_positions, p.wide = wide;
   p.n_slots = n_slots, p.eps = eps;
   const int rows = NR_UNROLL * 32 / (D / 8);
-  const int heads = H + Hkv * (to_cache ? 2 : 1);
-  const long long items = static_cast<long long>(T) * ((heads + rows - 1) / rows);
-  const int grid = static_cast<int>(std::min<long long>((items + NR_THREADS / 32 - 1) / (NR_THREADS / 32), sm_count() * 8ll));
-  auto kernel = D == 64 ? norm_rope_kernel<64> : D == 128 ? norm_rope_kernel<128> : norm_rope_kernel<256>;
+  const int chunks = (H + rows - 1) / rows + (to_cache ? 2 : 1) * ((Hkv + rows - 1) / rows);
+  const long long blocks = (static_cast<long long>(T) * chunks + NR_THREADS / 32 - 1) / (NR_THREADS / 32);
+  const int grid = static_cast<int>(std::min<long long>(blocks, sm_count() * NR_BLOCKS));
+  auto kernel = interleaved ? (D == 64 ? norm_rope_kernel<64, true> : D == 128 ? norm_rope_kernel<128, true> : norm_rope_kernel<256, true>)
+                            : (D == 64 ? norm_rope_kernel<64, false> : D == 128 ? norm_rope_kernel<128, false> : norm_rope_kernel<256, false>);
   kernel<<<grid, NR_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
   TJX_CUDA(cudaGetLastError());
   return 0;
