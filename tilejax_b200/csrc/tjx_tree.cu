@@ -500,13 +500,13 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
               if (!((see1 >> i) & 1)) v[1][i] = __float_as_uint(-INFINITY);
             }
           }
+          // (Maxima of two: 64 of them and the exponentials take two warps of a scheduler 830 cycles, 32 maxima of three 1030.)
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              mx[(i >> 1) & 3] = fmax3_nan(mx[(i >> 1) & 3], __uint_as_float(v[h][i]), __uint_as_float(v[h][i + 1]));
-          float m_blk = fmax_nan(fmax3_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2e;
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmax_nan(mx[i & 3], __uint_as_float(v[h][i]));
+          float m_blk = fmax_nan(fmax_nan(mx[0], mx[1]), fmax_nan(mx[2], mx[3])) * p.scale_log2e;
           if (m_blk == INFINITY) m_blk = NAN;
           if (last_job < 0) {
             m_used = fmax_nan(m_blk, TR_NOTHING);
