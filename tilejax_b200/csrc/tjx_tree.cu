@@ -295,7 +295,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  chain_release();
   const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_holder, 0);
   // (Through shuffles: the compiler must know that a warp's lanes walk together, or it keeps the issuers' addresses and
   // loop counters per lane.)
@@ -760,6 +759,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 }
 
 constexpr int TJ_WARPS = 8;
+constexpr int TJ_BATCH = 4;
 
 // The units that several CTAs shared: a CTA per 32 rows (a lane's) joins their partial results in the order of the
 // blocks, a warp 16 of the columns. And the rows that no unit has, which stay the query.
@@ -770,21 +770,30 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
   if (x < join.y * p.group) {
     const int first = blockIdx.x, n = join.w - first + 1;  // parts: 2 first + 1, 2 (first + 1), 2 (first + 2), ...
     auto part = [&](int i) { return static_cast<size_t>(2 * (first + i) + (i == 0 ? 1 : 0)); };
-    float m = TR_NOTHING;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.part_ml[part(i) * p.part_rows + x].x);
-    float sum = 0.f, o[16] = {};
-#pragma unroll 2
-    for (int i = 0; i < n; ++i) {
-      const float2 ml = p.part_ml[part(i) * p.part_rows + x];
-      const float w = ex2(ml.x - m);
-      sum = fmaf(w, ml.y, sum);
-      const float4* src = p.part_o + (part(i) * 32 + 4 * warp) * p.part_rows + x;
+    // TJ_BATCH parts' loads at a time, then their turn in order, the running maximum following.
+    float m = TR_NOTHING, sum = 0.f, o[16] = {};
+    for (int i0 = 0; i0 < n; i0 += TJ_BATCH) {
+      float2 ml[TJ_BATCH];
+      float4 v[TJ_BATCH][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 v = src[static_cast<size_t>(k) * p.part_rows];
-        o[4 * k] = fmaf(v.x, w, o[4 * k]), o[4 * k + 1] = fmaf(v.y, w, o[4 * k + 1]);
-        o[4 * k + 2] = fmaf(v.z, w, o[4 * k + 2]), o[4 * k + 3] = fmaf(v.w, w, o[4 * k + 3]);
+      for (int i = 0; i < TJ_BATCH; ++i) {
+        if (i0 + i >= n) break;
+        ml[i] = p.part_ml[part(i0 + i) * p.part_rows + x];
+        const float4* src = p.part_o + (part(i0 + i) * 32 + 4 * warp) * p.part_rows + x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = src[static_cast<size_t>(k) * p.part_rows];
+      }
+#pragma unroll
+      for (int i = 0; i < TJ_BATCH; ++i) {
+        if (i0 + i >= n) break;
+        const float m_new = fmaxf(m, ml[i].x), a = ex2(m - m_new), w = ex2(ml[i].x - m_new);
+        m = m_new;
+        sum = fmaf(sum, a, w * ml[i].y);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[4 * k] = fmaf(o[4 * k], a, v[i][k].x * w), o[4 * k + 1] = fmaf(o[4 * k + 1], a, v[i][k].y * w);
+          o[4 * k + 2] = fmaf(o[4 * k + 2], a, v[i][k].z * w), o[4 * k + 3] = fmaf(o[4 * k + 3], a, v[i][k].w * w);
+        }
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
