@@ -391,6 +391,77 @@ def test_tree_attention_refuses_what_it_cannot_do():
         ops.rpa_tree_attention(**{**dev, "q": wide[:4]}, out=wide[2:])
 
 
+def test_a_captured_step_follows_its_inputs():
+    # Captured once, replayed with other lengths, tables, masks and data in the same tensors; an eager call in between.
+    def case(seed, q_lens, kv_lens):
+        return tree_case(q_lens, kv_lens, 8, 2, 16, seed=seed, max_seqs=3, extra=40 - sum(q_lens), words=1, poison=False)
+
+    cases = [case(1, [20, 9, 3], [300, 1500, 77]), case(2, [4, 30], [4000, 31]), case(3, [1, 1, 1], [5, 1, 900])]
+    pool = max(len(c["kv_cache"]) for c in cases)
+    pps = max(len(c["page_indices"]) // 3 for c in cases)
+    for c in cases:
+        cache = np.zeros((pool, *c["kv_cache"].shape[1:]), BF16)
+        cache[: len(c["kv_cache"])] = c["kv_cache"]
+        table = np.zeros((3, pps), np.int32)
+        old = c["page_indices"].reshape(3, -1)
+        table[:, : old.shape[1]] = old
+        c["kv_cache"], c["page_indices"] = cache, table.reshape(-1)
+    dev = {k: to_device(v) for k, v in cases[0].items()}
+    ops.rpa_tree_attention(**dev, sm_scale=0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.rpa_tree_attention(**dev, sm_scale=0.1)
+    for c in (*cases, cases[0]):
+        for k, v in c.items():
+            dev[k].copy_(to_device(v))
+        graph.replay()
+        eager = ops.rpa_tree_attention(**dev, sm_scale=0.1)
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+        want, size = oracle.tree_attention_f64(*c.values(), 0.1)
+        close(to_host(out), want, size, 2.0**-8 + 2.0**-11)
+    assert ops.device_status() == 0
+
+
+def test_calls_on_two_streams_at_once():
+    cases = [{k: to_device(v) for k, v in tree_case([12, 30, 5], [3000, 900, 2000], 8, 2, 16, seed=s).items()} for s in (1, 2)]
+    alone = [ops.rpa_tree_attention(**c, sm_scale=0.1) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.rpa_tree_attention(**c, sm_scale=0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g.view(torch.int16), a.view(torch.int16)) for gs, a in zip(got, alone) for g in gs)
+
+
+def test_rows_behind_two_to_the_32_bytes():
+    # A cache of more than 2^31 elements, the sequences' pages at its end: write, attention and commit reach them.
+    page, kv_heads = 16, 8
+    pages = (1 << 31) // (page * kv_heads * 2 * 128) + 64
+    cache = torch.empty((pages, page, kv_heads, 2, 128), dtype=torch.bfloat16, device="cuda")
+    small = tree_case([9, 4], [150, 40], 16, kv_heads, page, seed=3, poison=False)
+    shift = pages - len(small["kv_cache"])
+    cache[shift:].copy_(to_device(small["kv_cache"]))
+    dev = {k: to_device(v) for k, v in small.items() if k != "kv_cache"}
+    low = {**dev, "kv_cache": to_device(small["kv_cache"])}
+    want = ops.rpa_tree_attention(**low, sm_scale=0.1)
+    dev["page_indices"] = dev["page_indices"] + shift
+    assert torch.equal(ops.rpa_tree_attention(**dev, kv_cache=cache, sm_scale=0.1).view(torch.int16), want.view(torch.int16))
+    paths, accepted = dev32([[0, 3, 5], [1, 2, 0]]), dev32([3, 2])
+    names = ("kv_lens", "page_indices", "cu_q_lens")
+    for c, d in ((cache, dev), (low["kv_cache"], low)):
+        ops.rpa_commit(c, *(d[n] for n in names), paths, accepted)
+    assert torch.equal(cache[shift:].view(torch.int16), low["kv_cache"].view(torch.int16))
+    k = to_device(rand_bf16((2, kv_heads, 128), 1))
+    slots = dev32([pages * page - 1, pages * page - 40])
+    ops.rpa_norm_rope_write(to_device(rand_bf16((2, 16, 128), 2)), k, k, None, None, dev32([0, 0]),
+                            torch.cat([torch.ones(1, 4), torch.zeros(1, 4)], 1).cuda(), cache, slots)
+    rows = cache.view(-1, kv_heads, 2, 128)
+    assert all(torch.equal(rows[int(s), :, i], k[t]) for t, s in enumerate(slots) for i in (0, 1))
+
+
 # ------------------------------------------------------------------------------------------ commit
 
 

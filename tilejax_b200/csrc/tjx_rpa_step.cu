@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(NR_THREADS, NR_BLOCKS) norm_rope_kernel(const 
 // ------------------------------------------------------------------------------------------ accepted path
 
 constexpr int COMMIT_THREADS = 256;
-constexpr int COMMIT_BATCH = 8;
+constexpr int COMMIT_BATCH = 16;
 
 // A CTA moves one sequence's accepted rows, each thread a 16-byte column of them, in path order and COMMIT_BATCH rows
 // at a time: all loads of a batch before its stores. The path's nodes ascend, so node d's row never lies in front of

@@ -50,7 +50,7 @@ constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a ga
 // (by their softmax, 1950), and what a unit takes beside its blocks: the last scores masked and their V rows looked at, the
 // pipeline drained, the rows out. Without the weights the CTA with the most units, or with the widest, ran a third longer
 // than the others (trees of 16 over 32 caches of up to 4096: 81 -> 66 us; of up to 64 over 64 of up to 8100: 340 -> 311).
-constexpr int TR_COST_ONE = 4, TR_COST_TWO = 6, TR_COST_UNIT = 24;
+constexpr int TR_COST_ONE = 4, TR_COST_TWO = 6, TR_COST_UNIT = 32;
 constexpr int TR_MIN_SHARE = 12;  // a run's cost, at least (it may not be shorter than a block)
 static_assert(TR_MIN_SHARE >= TR_COST_TWO && TR_MIN_SHARE >= TR_COST_ONE, "every run inside a unit has a block");
 
