@@ -9,6 +9,34 @@ import oracle
 from tilejax_b200 import ops
 
 
+@pytest.fixture(scope="module", autouse=True)
+def host_side(native):
+    """The operators' compiled host side (built on demand, as the library is)."""
+    from tilejax_b200.csrc.build import BINDING, build_binding
+
+    if not BINDING.exists():
+        build_binding()
+
+
+def test_the_host_side_names_itself_when_it_is_missing(monkeypatch):
+    import sys
+
+    import tilejax_b200
+
+    monkeypatch.setattr(ops, "_binding", None)
+    monkeypatch.setitem(sys.modules, "tilejax_b200._binding", None)
+    monkeypatch.delattr(tilejax_b200, "_binding", raising=False)
+    with pytest.raises(RuntimeError, match="csrc.build"):
+        ops.rpa_commit(None, None, None, None, None, None)
+
+
+def test_what_is_no_tensor_is_a_type_error():
+    with pytest.raises(TypeError, match="kv_lens must be a tensor"):
+        ops.rpa_commit(heads(4, 16, 2, 2, 128), [9, 4], i32(0, 1), i32(0, 1), i32(0)[None], i32(1))
+    with pytest.raises(TypeError):
+        ops.rpa_plan(i32(1), i32(1), i32(0), i32(0), i32(1), "4", 1)
+
+
 def i32(*values):
     return torch.tensor(values, dtype=torch.int32)
 
@@ -138,10 +166,3 @@ def test_commit_refusals():
         ("paths is", "paths", lambda t: t.long()),
         ("n_accepted", "n_accepted", lambda t: t[:1]),
     ])
-
-
-def test_overlap_is_seen_in_bytes():
-    base = torch.zeros(64, dtype=torch.int32)
-    assert ops._overlap(base[:10], base[9:]) and not ops._overlap(base[:10], base[10:])
-    assert ops._overlap(base.view(8, 8)[:, :2], base.view(8, 8)[:, 4:])  # ranges meet, though no element does
-    assert not ops._overlap(base[:0], base)

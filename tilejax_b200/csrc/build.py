@@ -76,6 +76,33 @@ def build(force: bool = False, verbose: bool = False, defines: tuple[str, ...] =
     return library
 
 
+BINDING = PACKAGE / "_binding.so"
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """Compile tjx_binding.cpp (the CPython host side of the drafted-step operators) into _binding.so in the package."""
+    source = CSRC / "tjx_binding.cpp"
+    if _stale(BINDING, [source, (CSRC / "../../include/tilejax_b200.h").resolve(), Path(__file__).resolve()]):
+        import sysconfig
+
+        import torch
+
+        root = Path(torch.__file__).resolve().parent
+        includes = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+                    Path(nvcc()).resolve().parent.parent / "include"]
+        fresh = BINDING.with_suffix(".so.new")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *[f"-I{i}" for i in includes], str(source), "-o", str(fresh), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        done = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if done.returncode != 0:
+            raise RuntimeError("g++ failed:\n" + done.stdout)
+        os.replace(fresh, BINDING)
+    return BINDING
+
+
 def ffi_include_dir() -> str | None:
     """Where jaxlib keeps the XLA FFI headers, or None where JAX is not installed."""
     try:
@@ -115,5 +142,7 @@ if __name__ == "__main__":
     output = Path(args.output).resolve() if args.output else None
     os.chdir(CSRC)
     print(build(args.force, args.verbose, tuple(args.defines), output))
+    if output is None:
+        print(build_binding(args.verbose))
     if args.ffi:
         print(build_ffi(args.verbose) or "jax.ffi.include_dir() is not available: the handler library was not built")

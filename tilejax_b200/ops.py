@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
-import struct
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -38,20 +37,6 @@ def _need_cuda(*tensors: torch.Tensor) -> torch.device:
         if not t.is_contiguous():
             raise ValueError("tensors must be contiguous (row-major)")
     return tensors[0].device
-
-
-def _launch(device: torch.device, entry: str, *args) -> None:
-    """A call into the library on `device`'s current stream: pointers as integers (None: null), the stream appended. The
-    current device is changed only if it is another one: a few microseconds that a small operator is not worth."""
-    index = device.index
-    call = getattr(library(), entry)
-    if torch._C._cuda_getDevice() == index:
-        code = call(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            code = call(*args, torch._C._cuda_getCurrentRawStream(index))
-    if code != 0:
-        check(code)
 
 
 _table_cache: dict[tuple, torch.Tensor] = {}
@@ -650,18 +635,25 @@ def ragged_paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
 
 # ------------------------------------------------------------------------------------------ a step over drafted tokens
 
-
-def _end(t: torch.Tensor) -> int:
-    """The address behind the last element."""
-    at = 1
-    for n, step in zip(t.shape, t.stride()):
-        at += (n - 1) * step
-    return t.data_ptr() + at * t.element_size()
+_binding = None
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from the first to the last element of the one meets that of the other."""
-    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < _end(b) and b.data_ptr() < _end(a)
+def _native():
+    """The CPython host side of the operators below (csrc/tjx_binding.cpp): it checks their arguments, allocates and calls
+    the C ABI; refusals are ValueError, the library's errors NativeError."""
+    global _binding
+    if _binding is None:
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise RuntimeError("tilejax_b200/_binding.so is missing or of another Python or torch: build it with "
+                               "`python -m tilejax_b200.csrc.build`") from e
+        lib = library()
+        entries = (lib.tjx_rpa_plan, lib.tjx_norm_rope_bf16, lib.tjx_rpa_tree_attention_workspace_bytes,
+                   lib.tjx_rpa_tree_attention_bf16, lib.tjx_rpa_commit_bf16)
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), check)
+        _binding = module
+    return _binding
 
 
 class RpaStep(NamedTuple):
@@ -683,130 +675,11 @@ def rpa_plan(ctx_lens: torch.Tensor, q_lens: torch.Tensor, page_indices: torch.T
     all at most `tokens` rows. The pages it lacks come off the top of the stack free_pages[: n_free[0]], sequence after
     sequence, and are entered in page_indices (S * pages_per_seq,) IN PLACE behind those it holds, -1 where the stack
     is empty. `depths` (tokens,) gives drafted tokens their depth in the tree: the token's position is then ctx_lens[s]
-    plus its depth, while its slot stays that of its index. `out` is written instead of new tensors; it may not overlap
-    the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into ctx_lens)."""
-    inputs = [ctx_lens, q_lens, page_indices, free_pages, n_free]
-    shapes = [t.shape for t in inputs]
-    for name, t, shape in zip(("ctx_lens", "q_lens", "page_indices", "free_pages", "n_free"), inputs, shapes):
-        if t.dtype is not torch.int32 or len(shape) != 1:
-            raise ValueError(f"{name} must be an int32 vector")
-    (S,), (S_new,), (entries,), (capacity,), (counts,) = shapes
-    T = int(tokens)
-    if S == 0 or S_new != S or entries == 0 or entries % S:
-        raise ValueError("ctx_lens and q_lens are (S,), page_indices (S * pages_per_seq,)")
-    if counts < 1:
-        raise ValueError("n_free holds the number of free pages")
-    held_ptr = depths_ptr = None
-    if pages_held is not None:
-        inputs.append(pages_held)
-        held_ptr = pages_held.data_ptr()
-        if pages_held.shape != (S,) or pages_held.dtype is not torch.int32:
-            raise ValueError("pages_held is int32 (S,)")
-    if depths is not None:
-        inputs.append(depths)
-        depths_ptr = depths.data_ptr()
-        if depths.shape != (T,) or depths.dtype is not torch.int32:
-            raise ValueError("depths is int32 (tokens,)")
-    if T < 0 or page_size <= 0:
-        raise ValueError("page_size must be positive and tokens not negative")
-    device = _need_cuda(*inputs)
-    if out is None:
-        block = torch.empty(3 * S + 3 + 2 * T, dtype=torch.int32, device=device)
-        out = RpaStep._make(block.split_with_sizes((S, S + 1, T, T, S, 2)))
-        at = block.data_ptr()
-        outputs = (at, at + 4 * S, at + 8 * S + 4, at + 8 * S + 4 + 4 * T, at + 8 * S + 4 + 8 * T, at + 12 * S + 4 + 8 * T)
-    else:
-        _need_cuda(ctx_lens, *out)
-        if [tuple(t.shape) for t in out] != [(S,), (S + 1,), (T,), (T,), (S,), (2,)] or any(t.dtype is not torch.int32 for t in out):
-            raise ValueError("out is a step of other sizes")
-        if any(_overlap(a, b) for a in out for b in inputs):
-            raise ValueError("out overlaps an input")
-        outputs = [t.data_ptr() for t in out]
-    _launch(device, "tjx_rpa_plan", ctx_lens.data_ptr(), q_lens.data_ptr(), held_ptr, depths_ptr, page_indices.data_ptr(),
-            free_pages.data_ptr(), n_free.data_ptr(), capacity, S, T, entries // S, page_size, *outputs)
-    return out
-
-
-_pack_strides = struct.Struct("10q").pack
-
-
-def _heads(name: str, t: torch.Tensor, tokens: int, D: int) -> tuple[int, int, int, int]:
-    """Heads, token stride, head stride and address of a (tokens, heads, D) operand."""
-    shape = t.shape
-    if len(shape) != 3 or t.dtype is not torch.bfloat16 or shape[0] != tokens or shape[2] != D:
-        raise ValueError(f"{name} must be bfloat16 ({tokens}, heads, {D})")
-    token, head, dense = t.stride()
-    at = t.data_ptr()
-    if dense != 1 or (token | head) & 3 or at & 7:
-        raise ValueError(f"{name}'s last dimension must be dense, its strides multiples of 4 elements, its data 8-byte aligned")
-    return shape[1], token, head, at
-
-
-def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a is b or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride())
-
-
-def _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, kv_cache, slots, eps, interleaved):
-    shape = q.shape
-    if len(shape) != 3:
-        raise ValueError("q is (T, H, D)")
-    T, H, D = shape
-    _, q_tok, q_head, q_at = _heads("q", q, T, D)
-    Hkv, k_tok, k_head, k_at = _heads("k", k, T, D)
-    v_tok = v_head = n_slots = ko_tok = ko_head = 0
-    v_at = qg_at = kg_at = slots_at = ko_at = cache_at = None
-    dense = [positions, cos_sin]
-    if q_gamma is not None and k_gamma is not None:
-        dense += (q_gamma, k_gamma)
-        qg_at, kg_at = q_gamma.data_ptr(), k_gamma.data_ptr()
-        if q_gamma.shape != (D,) or k_gamma.shape != (D,) or q_gamma.dtype is not torch.bfloat16 \
-                or k_gamma.dtype is not torch.bfloat16 or (qg_at | kg_at) & 7:
-            raise ValueError(f"the gammas are bfloat16 ({D},), 8-byte aligned")
-    elif q_gamma is not k_gamma:
-        raise ValueError("q_gamma and k_gamma are given together or not at all")
-    if positions.shape != (T,) or positions.dtype is not torch.int32:
-        raise ValueError("positions is int32 (T,)")
-    table, table_at = cos_sin.shape, cos_sin.data_ptr()
-    if len(table) != 2 or cos_sin.dtype is not torch.float32 or table[1] > D or table[1] & 7 or table[0] == 0 or table_at & 15:
-        raise ValueError("cos_sin is float32 (max_positions, rot), rot a multiple of 8 up to the head dimension, 16-byte aligned")
-    used = [q, k]
-    if kv_cache is not None:
-        used.append(v)
-        _, v_tok, v_head, v_at = _heads("v", v, T, D)
-        dense += (slots, kv_cache)
-        slots_at, cache_at, n_slots = slots.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0] * kv_cache.shape[1]
-    device = _need_cuda(*dense)
-    index = device.index
-    for t in used:
-        if t.get_device() != index:
-            raise ValueError("all tensors must be on the same device")
-    if q_out is None:
-        q_out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-        qo_tok, qo_head, qo_at = H * D, D, q_out.data_ptr()
-    else:
-        heads, qo_tok, qo_head, qo_at = _heads("the queries' output", q_out, T, D)
-        if heads != H or q_out.device != device or any(_overlap(q_out, t) for t in used if not _same(q_out, q)):
-            raise ValueError("the queries' output is q itself or memory of its own, like q")
-    if kv_cache is not None:
-        behind = cache_at + 2 * n_slots * 2 * Hkv * D
-        for at, heads, token, head in ((q_at, H, q_tok, q_head), (k_at, Hkv, k_tok, k_head), (v_at, Hkv, v_tok, v_head),
-                                       (qo_at, H, qo_tok, qo_head)):
-            if at < behind and at + 2 * ((T - 1) * token + (heads - 1) * head + D) > cache_at:
-                raise ValueError("the cache overlaps an operand")
-    elif k_out is None:
-        k_out = torch.empty((T, Hkv, D), dtype=torch.bfloat16, device=device)
-        ko_tok, ko_head, ko_at = Hkv * D, D, k_out.data_ptr()
-    else:
-        heads, ko_tok, ko_head, ko_at = _heads("the keys' output", k_out, T, D)
-        if heads != Hkv or k_out.device != device or any(_overlap(k_out, t) for t in (q, k, q_out) if not _same(k_out, k)):
-            raise ValueError("the keys' output is k itself or memory of its own, like k")
-    if T == 0:
-        return q_out, k_out
-    _launch(device, "tjx_norm_rope_bf16", q_at, k_at, v_at,
-            _pack_strides(q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head), qg_at, kg_at,
-            positions.data_ptr(), table_at, slots_at, qo_at, ko_at, cache_at, T, H, Hkv, D, table[1], table[0],
-            1 if interleaved else 0, n_slots, eps)
-    return q_out, k_out
+    plus its depth, while its slot stays that of its index. All tensors are int32 vectors. `out` is written instead of
+    new tensors; it may not overlap the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into
+    ctx_lens)."""
+    return RpaStep._make(_native().rpa_plan(ctx_lens, q_lens, page_indices, free_pages, n_free, page_size, tokens,
+                                            pages_held, depths, out))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None,
@@ -818,8 +691,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_gamma: torch.Tensor | None,
     (max_positions, rot); positions past the table are clamped to it). Pair i is elements i and i + rot / 2, or 2 i and
     2 i + 1 if `interleaved`. q and k may be views of one projection's output: any token and head strides that are
     multiples of 4. Returns (q', k'); out=(q, k) updates in place. D 64, 128 or 256."""
-    q_out, k_out = out if out is not None else (None, None)
-    return _norm_rope(q, k, None, q_gamma, k_gamma, positions, cos_sin, q_out, k_out, None, None, eps, interleaved)
+    q_out, k_out = (None, None) if out is None else out
+    return _native().norm_rope(q, k, None, q_gamma, k_gamma, positions, cos_sin, None, None, eps, interleaved, q_out, k_out)
 
 
 def rpa_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gamma: torch.Tensor | None,
@@ -829,22 +702,10 @@ def rpa_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_gam
     """`qk_norm_rope` with the cache write in the same pass: the turned key and the value of token t go to row slots[t]
     (page * page_size + row, as `rpa_plan` gives it; out of range: not written; no slot twice) of the cache
     (pages, page_size, Hkv, 2, D), IN PLACE. Returns (q', the cache); `out=q` updates the queries in place."""
-    cache, q_shape, k_shape = kv_cache.shape, q.shape, k.shape
-    if len(cache) != 5 or cache[3] != 2 or kv_cache.dtype is not torch.bfloat16 or 0 in cache:
+    if kv_cache is None:
         raise ValueError("the cache is (pages, page_size, Hkv, 2, D) bfloat16: each head's key and value side by side")
-    if len(q_shape) != 3 or k_shape != (q_shape[0], cache[2], cache[4]) or v.shape != k_shape:
-        raise ValueError("q is (T, H, D), k and v (T, Hkv, D) with the cache's Hkv and D")
-    if cache[0] * cache[1] >= 1 << 31:
-        raise ValueError("the cache's rows must fit in int32")
-    if slots.shape != (q_shape[0],) or slots.dtype is not torch.int32:
-        raise ValueError("slots is int32 (T,)")
-    q_out, _ = _norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, out, None, kv_cache, slots, eps, interleaved)
-    return q_out, kv_cache
-
-
-@lru_cache(maxsize=256)
-def _tree_workspace_bytes(T: int, S: int, H: int, Hkv: int) -> int:
-    return int(library().tjx_rpa_tree_attention_workspace_bytes(T, S, H, Hkv))
+    return _native().norm_rope(q, k, v, q_gamma, k_gamma, positions, cos_sin, kv_cache, slots, eps, interleaved, out,
+                               None)[0], kv_cache
 
 
 def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor,
@@ -856,30 +717,7 @@ def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.T
     (bit j % 32 of word j // 32) is set in tree_mask[t], int32 (T, words): its ancestors and itself. Their rows become
     the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
     the sequences from distribution[0] on. `out=q` updates in place."""
-    num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
-    if q.dim() != 3 or q.shape[2] != D or q.dtype is not torch.bfloat16:
-        raise ValueError("q is (T, H, D) bfloat16")
-    T, H, _ = q.shape
-    if cu_q_lens.shape != (S + 1,) or distribution.shape != (3,) or cu_q_lens.dtype is not torch.int32 \
-            or distribution.dtype is not torch.int32:
-        raise ValueError("cu_q_lens is int32 (S + 1,), distribution int32 (3,)")
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.shape[1] == 0 or tree_mask.dtype is not torch.int32:
-        raise ValueError("tree_mask is int32 (T, words), 32 new tokens a word")
-    device = _need_cuda(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution)
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
-        raise ValueError("out must look like q")
-    elif out.data_ptr() != q.data_ptr() and _overlap(out, q):
-        raise ValueError("out is q itself or memory of its own")
-    if T == 0:
-        return out
-    need = _tree_workspace_bytes(T, S, H, Hkv)
-    ws = torch.empty(need + 256, dtype=torch.uint8, device=device)  # (of the stream it is used on: no other may get it early)
-    _launch(device, "tjx_rpa_tree_attention_bf16", q.data_ptr(), out.data_ptr(), kv_cache.data_ptr(), kv_lens.data_ptr(),
-            page_indices.data_ptr(), cu_q_lens.data_ptr(), tree_mask.data_ptr(), distribution.data_ptr(), T, S, H, Hkv, D,
-            tree_mask.shape[1], page_size, pps, num_pages, sm_scale, (ws.data_ptr() + 255) & ~255, need)
-    return out
+    return _native().rpa_tree_attention(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution, sm_scale, out)
 
 
 def rpa_commit(kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torch.Tensor, cu_q_lens: torch.Tensor,
@@ -889,23 +727,7 @@ def rpa_commit(kv_cache: torch.Tensor, kv_lens: torch.Tensor, page_indices: torc
     IN PLACE, and the sequence's length becomes those positions and the accepted tokens; n_accepted[s] < 0 keeps all
     its tokens. A path ends in front of an entry that does not ascend or is no new token. Returns the lengths, int32
     (S,), `out` if given (not kv_lens itself)."""
-    num_pages, page_size, Hkv, D, S, pps = _rpa_sizes(kv_cache, kv_lens, page_indices)
-    if cu_q_lens.shape != (S + 1,) or cu_q_lens.dtype is not torch.int32:
-        raise ValueError("cu_q_lens is int32 (S + 1,)")
-    if paths.dim() != 2 or paths.shape[0] != S or paths.shape[1] == 0 or paths.dtype is not torch.int32 \
-            or n_accepted.shape != (S,) or n_accepted.dtype is not torch.int32:
-        raise ValueError("paths is int32 (S, P), n_accepted int32 (S,)")
-    device = _need_cuda(kv_cache, kv_lens, page_indices, cu_q_lens, paths, n_accepted)
-    if out is None:
-        out = torch.empty(S, dtype=torch.int32, device=device)
-    elif out.shape != (S,) or out.dtype is not torch.int32 or not out.is_contiguous() or out.device != device:
-        raise ValueError("out is int32 (S,), on the cache's device")
-    elif any(_overlap(out, t) for t in (kv_lens, page_indices, cu_q_lens, paths, n_accepted)):
-        raise ValueError("out overlaps an input")
-    _launch(device, "tjx_rpa_commit_bf16", kv_cache.data_ptr(), kv_lens.data_ptr(), page_indices.data_ptr(),
-            cu_q_lens.data_ptr(), paths.data_ptr(), n_accepted.data_ptr(), out.data_ptr(), S, paths.shape[1], Hkv, D,
-            page_size, pps, num_pages)
-    return out
+    return _native().rpa_commit(kv_cache, kv_lens, page_indices, cu_q_lens, paths, n_accepted, out)
 
 
 def paged_gqa_decode_static(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_tables: torch.Tensor,
