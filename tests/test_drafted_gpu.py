@@ -465,12 +465,12 @@ def test_rows_behind_two_to_the_32_bytes():
 # ------------------------------------------------------------------------------------------ commit
 
 
-def test_commit_is_exact():
+@pytest.mark.parametrize(("kv_heads", "page"), [(3, 16), (1, 48), (12, 32)])
+def test_commit_is_exact(kv_heads, page):
     rng = np.random.default_rng(4)
-    kv_heads, page = 3, 16
-    for seed, (q_lens, kv_lens) in enumerate([([5], [5]), ([1, 16, 64, 9, 4, 40], [30, 100, 64, 10, 4, 300])]):
-        inp = tree_case(q_lens, kv_lens, 3, kv_heads, page, seed=seed, poison=False)
-        P = 24
+    for seed, (q_lens, kv_lens) in enumerate([([5], [5]), ([1, 16, 64, 9, 4, 40, 70], [30, 100, 64, 10, 4, 300, 200])]):
+        inp = tree_case(q_lens, kv_lens, kv_heads, kv_heads, page, seed=seed, poison=False)
+        P = 40
         paths = np.stack([np.sort(rng.permutation(80)[:P]) for _ in q_lens]).astype(np.int32)
         for s, n in enumerate(q_lens):
             take = min(n, P)
