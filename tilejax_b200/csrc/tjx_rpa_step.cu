@@ -17,7 +17,7 @@ namespace tjx {
 // ------------------------------------------------------------------------------------------ block tables and slots
 
 constexpr int PLAN_THREADS = 1024;
-constexpr int PLAN_MAX_SEQS = 8192;  // two int32 prefix arrays in shared memory
+constexpr int PLAN_MAX_SEQS = 8192;  // 16 bytes of shared memory each
 
 struct PlanParams {
   const int32_t *ctx_lens, *q_lens, *held, *depths;  // held, depths: or null
@@ -28,132 +28,138 @@ struct PlanParams {
   int32_t *kv_lens, *cu_q_lens, *positions, *slots, *held_out, *n_free_out;
 };
 
-// Last entry of the nondecreasing prefix array a[0..n) that is <= x (a[0] <= x).
-__device__ __forceinline__ int prefix_find(const int* a, int n, int x) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a[mid] <= x) lo = mid; else hi = mid;
+// A sequence as the scan leaves it in shared memory.
+struct PlanSeq {
+  int first, lack;  // its first token (clipped to T), its first fresh page
+  int ctx, held;
+};
+
+// Inclusive sums over the CTA's threads, and the sums of all of them. `sums` is not reused before a __syncthreads.
+struct PlanSums {
+  long long q[32];
+  int n[32];
+};
+__device__ __forceinline__ void plan_scan(PlanSums& sums, long long& q, int& n, long long& all_q, int& all_n) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long yq = __shfl_up_sync(0xFFFFFFFFu, q, d);
+    const int yn = __shfl_up_sync(0xFFFFFFFFu, n, d);
+    if (lane >= d) q += yq, n += yn;
   }
-  return lo;
+  if (lane == 31) sums.q[warp] = q, sums.n[warp] = n;
+  __syncthreads();
+  long long wq = sums.q[lane];  // every warp adds the warps' sums up for itself
+  int wn = sums.n[lane];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long yq = __shfl_up_sync(0xFFFFFFFFu, wq, d);
+    const int yn = __shfl_up_sync(0xFFFFFFFFu, wn, d);
+    if (lane >= d) wq += yq, wn += yn;
+  }
+  all_q = __shfl_sync(0xFFFFFFFFu, wq, 31), all_n = __shfl_sync(0xFFFFFFFFu, wn, 31);
+  const long long bq = __shfl_sync(0xFFFFFFFFu, wq, max(warp - 1, 0));
+  const int bn = __shfl_sync(0xFFFFFFFFu, wn, max(warp - 1, 0));
+  if (warp > 0) q += bq, n += bn;
 }
 
-// Every CTA scans all sequences (new tokens, and pages a sequence lacks) into shared memory and then takes its share
-// of the tokens and of the pages handed out; CTA 0 also writes what there is one of per sequence. Nothing a CTA reads
-// is written by another: table entries below a sequence's held pages are only read, those handed out only written
-// (a token on such a page takes it from the free list itself). Bound by latency: a load, a scan, a search and two
-// dependent loads.
-__global__ void __launch_bounds__(PLAN_THREADS) rpa_plan_kernel(const PlanParams p) {
-  extern __shared__ int plan_smem[];
-  int* cu = plan_smem;            // [S + 1] first token of each sequence, clipped to T
-  int* lack = plan_smem + p.S + 1;  // [S + 1] first fresh page of each sequence
-  __shared__ long long warp_q[32];
-  __shared__ int warp_n[32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  long long carry_q = 0;
-  int carry_n = 0;
+// Every CTA scans all sequences (new tokens, and pages a sequence lacks) into shared memory and then takes its share of
+// the tokens and of the pages handed out; CTA 0 also writes what there is one of per sequence. Nothing a CTA reads is
+// written by another: table entries below a sequence's held pages are only read, those handed out only written (a token on
+// such a page takes it from the free list itself). Bound by latency: a load, a scan, a search and a load more.
+__global__ void __launch_bounds__(PLAN_THREADS, 2) rpa_plan_kernel(const PlanParams p) {
+  extern __shared__ __align__(16) uint8_t plan_smem[];
+  PlanSeq* seq = reinterpret_cast<PlanSeq*>(plan_smem);  // [S + 1], the last: all tokens, all fresh pages
+  __shared__ PlanSums sums[2];
+  const int t = threadIdx.x;
   const int free_now = min(max(p.n_free[0], 0), p.free_capacity);
-  for (int s0 = 0; s0 < p.S; s0 += PLAN_THREADS) {
+  auto lacking = [&](int ctx, int held, long long tokens) {
+    const long long len = min(static_cast<long long>(ctx) + tokens, 0x7FFFFFFFll);
+    const unsigned pages = (static_cast<unsigned>(len) + static_cast<unsigned>(p.page_size) - 1u) / static_cast<unsigned>(p.page_size);
+    return max(static_cast<int>(min(pages, static_cast<unsigned>(p.pages_per_seq))) - held, 0);
+  };
+  long long tokens = 0;  // of the sequences before
+  int fresh_pages = 0;
+  for (int s0 = 0, round = 0; s0 < p.S; s0 += PLAN_THREADS, ++round) {
     const int s = s0 + t;
-    int q = 0, need = 0, ctx = 0, held = 0;
+    PlanSeq me{0, 0, 0, 0};
+    long long q = 0;
+    int n = 0;
     if (s < p.S) {
-      ctx = max(p.ctx_lens[s], 0), q = max(p.q_lens[s], 0);
-      const int cached = static_cast<int>((static_cast<long long>(ctx) + p.page_size - 1) / p.page_size);
-      held = min(max(p.held != nullptr ? p.held[s] : cached, 0), p.pages_per_seq);
+      me.ctx = max(p.ctx_lens[s], 0), q = max(p.q_lens[s], 0);
+      const unsigned cached = (static_cast<unsigned>(me.ctx) + static_cast<unsigned>(p.page_size) - 1u) / static_cast<unsigned>(p.page_size);
+      const int held = p.held != nullptr ? p.held[s] : static_cast<int>(min(cached, static_cast<unsigned>(p.pages_per_seq)));
+      me.held = min(max(held, 0), p.pages_per_seq);
+      n = lacking(me.ctx, me.held, q);
     }
-    // The scan of the new tokens comes first: a sequence past row T adds what fits.
-    long long iq = q;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xFFFFFFFFu, iq, d);
-      if (lane >= d) iq += y;
-    }
-    if (lane == 31) warp_q[warp] = iq;
-    __syncthreads();
-    if (warp == 0) {
-      long long w = warp_q[lane];
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(0xFFFFFFFFu, w, d);
-        if (lane >= d) w += y;
-      }
-      warp_q[lane] = w;
-    }
-    __syncthreads();
-    const long long end_q = carry_q + (warp > 0 ? warp_q[warp - 1] : 0) + iq;
-    const int first = static_cast<int>(min(end_q - q, static_cast<long long>(p.T)));
-    const int last = static_cast<int>(min(end_q, static_cast<long long>(p.T)));
-    const int len = static_cast<int>(min(static_cast<long long>(ctx) + (last - first), 0x7FFFFFFFll));
-    if (s < p.S) {
-      const long long pages = (static_cast<long long>(len) + p.page_size - 1) / p.page_size;
-      need = max(static_cast<int>(min(pages, static_cast<long long>(p.pages_per_seq))) - held, 0);
-    }
-    int in = need;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xFFFFFFFFu, in, d);
-      if (lane >= d) in += y;
-    }
-    if (lane == 31) warp_n[warp] = in;
-    __syncthreads();
-    if (warp == 0) {
-      int w = warp_n[lane];
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xFFFFFFFFu, w, d);
-        if (lane >= d) w += y;
-      }
-      warp_n[lane] = w;
-    }
-    __syncthreads();
-    const int before = carry_n + (warp > 0 ? warp_n[warp - 1] : 0) + in - need;
-    if (s < p.S) {
-      cu[s] = first;
-      lack[s] = before;
-      if (blockIdx.x == 0) {
-        p.kv_lens[s] = len;
-        p.cu_q_lens[s] = first;
-        p.held_out[s] = held + min(max(free_now - before, 0), need);
-      }
-    }
-    carry_q += warp_q[31];
-    carry_n += warp_n[31];
-    __syncthreads();  // the warps' sums are overwritten by the next round
+    long long upto_q = q, all_q;
+    int upto_n = n, all_n;
+    plan_scan(sums[round & 1], upto_q, upto_n, all_q, all_n);
+    me.first = static_cast<int>(min(tokens + upto_q - q, static_cast<long long>(p.T)));
+    me.lack = fresh_pages + upto_n - n;
+    if (s < p.S) seq[s] = me;
+    tokens += all_q, fresh_pages += all_n;
   }
-  const int total = static_cast<int>(min(carry_q, static_cast<long long>(p.T)));
-  if (t == 0) {
-    cu[p.S] = total, lack[p.S] = carry_n;
-    if (blockIdx.x == 0) {
-      p.cu_q_lens[p.S] = total;
-      p.n_free_out[0] = max(free_now - carry_n, 0);
-      p.n_free_out[1] = max(carry_n - free_now, 0);
-    }
-  }
+  const int total = static_cast<int>(min(tokens, static_cast<long long>(p.T)));
+  if (t == 0) seq[p.S] = PlanSeq{total, fresh_pages, 0, 0};
   __syncthreads();
+  if (tokens > p.T) {  // rows for some of the tokens only: the pages again, for those
+    fresh_pages = 0;
+    for (int s0 = 0, round = 0; s0 < p.S; s0 += PLAN_THREADS, ++round) {
+      const int s = s0 + t;
+      long long q = 0, all_q;
+      int n = s < p.S ? lacking(seq[s].ctx, seq[s].held, seq[s + 1].first - seq[s].first) : 0, all_n;
+      int upto_n = n;
+      __syncthreads();
+      plan_scan(sums[round & 1], q, upto_n, all_q, all_n);
+      if (s < p.S) seq[s].lack = fresh_pages + upto_n - n;
+      fresh_pages += all_n;
+    }
+    if (t == 0) seq[p.S].lack = fresh_pages;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0) {
+    for (int s = t; s < p.S; s += PLAN_THREADS) {
+      const PlanSeq me = seq[s];
+      const int lacks = seq[s + 1].lack - me.lack;
+      p.kv_lens[s] = static_cast<int>(min(static_cast<long long>(me.ctx) + (seq[s + 1].first - me.first), 0x7FFFFFFFll));
+      p.cu_q_lens[s] = me.first;
+      p.held_out[s] = me.held + min(max(free_now - me.lack, 0), lacks);
+    }
+    if (t == 0) {
+      p.cu_q_lens[p.S] = total;
+      p.n_free_out[0] = max(free_now - fresh_pages, 0);
+      p.n_free_out[1] = max(fresh_pages - free_now, 0);
+    }
+  }
   const int step = static_cast<int>(gridDim.x) * PLAN_THREADS, me = static_cast<int>(blockIdx.x) * PLAN_THREADS + t;
-  auto held_of = [&](int s) {
-    const int cached = static_cast<int>((static_cast<long long>(max(p.ctx_lens[s], 0)) + p.page_size - 1) / p.page_size);
-    return min(max(p.held != nullptr ? p.held[s] : cached, 0), p.pages_per_seq);
+  // The last sequence that starts at or before x, by its first token or its first fresh page.
+  auto find = [&](auto key, int x) {
+    int lo = 0, hi = p.S + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (key(seq[mid]) <= x) lo = mid; else hi = mid;
+    }
+    return lo;
   };
   // The k-th page handed out comes off the top of the free stack, or is missing.
   auto fresh = [&](int k) { return k < free_now ? p.free_pages[free_now - 1 - k] : -1; };
-  for (int k = me; k < carry_n; k += step) {
-    const int s = prefix_find(lack, p.S + 1, k);
-    p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + held_of(s) + (k - lack[s])] = fresh(k);
+  for (int k = me; k < fresh_pages; k += step) {
+    const int s = find([](const PlanSeq& x) { return x.lack; }, k);
+    p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + seq[s].held + (k - seq[s].lack)] = fresh(k);
   }
   for (int i = me; i < p.T; i += step) {
     int position = 0, slot = -1;
     if (i < total) {
-      const int s = prefix_find(cu, p.S + 1, i);
-      const int ctx = max(p.ctx_lens[s], 0), index = i - cu[s];
-      const unsigned place = static_cast<unsigned>(ctx) + static_cast<unsigned>(index);
-      const unsigned page = place / static_cast<unsigned>(p.page_size), row = place % static_cast<unsigned>(p.page_size);
-      position = p.depths != nullptr ? ctx + p.depths[i] : static_cast<int>(place);
+      const int s = find([](const PlanSeq& x) { return x.first; }, i);
+      const PlanSeq of = seq[s];
+      const unsigned place = static_cast<unsigned>(of.ctx) + static_cast<unsigned>(i - of.first);
+      const unsigned page = place / static_cast<unsigned>(p.page_size), row = place - page * static_cast<unsigned>(p.page_size);
+      position = p.depths != nullptr ? of.ctx + p.depths[i] : static_cast<int>(place);
       if (page < static_cast<unsigned>(p.pages_per_seq)) {
-        const int held = held_of(s);
-        const int entry = static_cast<int>(page) < held
+        const int entry = static_cast<int>(page) < of.held
                               ? p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + page]
-                              : fresh(lack[s] + static_cast<int>(page) - held);
+                              : fresh(of.lack + static_cast<int>(page) - of.held);
         if (entry >= 0) slot = entry * p.page_size + static_cast<int>(row);
       }
     }
@@ -437,15 +443,16 @@ int tjx_rpa_plan(const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* 
   p.S = S, p.T = T, p.pages_per_seq = pages_per_seq, p.page_size = page_size;
   p.kv_lens = kv_lens, p.cu_q_lens = cu_q_lens, p.positions = positions, p.slots = slots;
   p.held_out = pages_held_out, p.n_free_out = n_free_out;
-  const size_t smem = 2 * static_cast<size_t>(S + 1) * sizeof(int);
+  const size_t smem = static_cast<size_t>(S + 1) * sizeof(PlanSeq);
   static bool configured[64] = {};
   int dev = 0;
   TJX_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    TJX_CUDA(cudaFuncSetAttribute(rpa_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (PLAN_MAX_SEQS + 1) * 4));
+    TJX_CUDA(cudaFuncSetAttribute(rpa_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>((PLAN_MAX_SEQS + 1) * sizeof(PlanSeq))));
     configured[dev & 63] = true;
   }
-  const int grid = std::max(1, std::min((T + PLAN_THREADS - 1) / PLAN_THREADS, sm_count()));
+  const int grid = std::max(1, std::min((T + PLAN_THREADS - 1) / PLAN_THREADS, 2 * sm_count()));
   rpa_plan_kernel<<<grid, PLAN_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(p);
   TJX_CUDA(cudaGetLastError());
   return 0;
