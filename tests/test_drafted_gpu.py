@@ -82,6 +82,23 @@ def test_plan_refuses_an_output_among_its_inputs():
         ops.rpa_plan(dev32([0] * S), dev32([1] * S), dev32([0] * S), dev32([0]), dev32([1]), 4, S)
 
 
+def test_plan_refuses_a_table_among_its_other_inputs_and_outputs_in_one_place():
+    both = dev32([0, -1, 1, -1, 2, 3])
+    args = (dev32([3, 4]), dev32([1, 1]), both[:4], both[3:], dev32([2]), 4, 2)
+    with pytest.raises(ValueError, match="page_indices overlaps"):
+        ops.rpa_plan(*args)
+    args = (*args[:3], both[4:], *args[4:])
+    step = ops.rpa_plan(*args)
+    with pytest.raises(ValueError, match="out's tensors overlap"):
+        ops.rpa_plan(*args, out=step._replace(slots=step.positions))
+
+
+def test_a_table_entry_past_the_last_slot_has_none():
+    # 2^31 - 1 and 2^29 are no pages of a cache whose rows fit int32; their slots must not wrap round to some that are.
+    step = ops.rpa_plan(dev32([3, 3, 3]), dev32([1, 1, 1]), dev32([2**31 - 1, 2**29, 2**29 - 1]), dev32([0]), dev32([0]), 4, 3)
+    assert to_host(step.slots).tolist() == [-1, -1, 2**31 - 1]
+
+
 # ------------------------------------------------------------------------------------------ norm, rotation, write
 
 
@@ -187,6 +204,35 @@ def test_norm_and_rotation_refuse_overlapping_outputs_and_unknown_heads():
                          torch.zeros(4, 32, device="cuda"))
     with pytest.raises(NativeError, match="eps"):
         ops.qk_norm_rope(q, k, *args, eps=float("nan"))
+
+
+def test_norm_and_rotation_into_views_of_one_tensor():
+    # Outputs side by side within a token, and head by head, are apart; in place they are what separate ones are.
+    rng = np.random.default_rng(3)
+    T, D = 37, 64
+    table, where = torch.from_numpy(angles(50, D)).cuda(), dev32(rng.integers(0, 50, T))
+    gammas = [torch.from_numpy(rng.normal(1, 0.1, D)).to("cuda", torch.bfloat16) for _ in range(2)]
+    packed = torch.from_numpy(rng.normal(size=(T, 14, D))).to("cuda", torch.bfloat16)
+    for cut in (lambda x: (x[:, :9], x[:, 9:13]), lambda x: (x[:, ::2], x[:, 1::2])):
+        q, k = cut(packed)
+        want = ops.qk_norm_rope(q.contiguous(), k.contiguous(), *gammas, where, table)
+        into = torch.full_like(packed, 7)
+        got = ops.qk_norm_rope(q, k, *gammas, where, table, out=cut(into))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and (into[:, 13:] == 7).all() == (q.shape[1] == 9)
+        place = packed.clone()
+        got = ops.qk_norm_rope(*cut(place), *gammas, where, table, out=cut(place))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_norm_and_rotation_refuse_operands_that_share_elements():
+    x = torch.zeros(4, 8, 128, dtype=torch.bfloat16, device="cuda")
+    rest = (None, None, dev32([0] * 4), torch.zeros(4, 128, device="cuda"))
+    one = x[:1].expand(4, 8, 128)
+    for q, k, out in [(x, x, (x, x)), (x[:, :5], x[:, 4:], (x[:, :5], x[:, 4:])),  # in place, a head of both
+                      (x, x[:, :2].clone(), (one, x[:, :2].clone())), (one, x[:, :2].clone(), (one, x[:, :2].clone())),
+                      (x[:, :2], x[:, 2:4], (x[:, 4:6], x[:, 5:7])), (x[:, ::2], x[:, 1::2], (x[:, ::2], x[:, :4]))]:
+        with pytest.raises(ValueError, match="memory of its own"):
+            ops.qk_norm_rope(q, k, *rest, out=out)
 
 
 # ------------------------------------------------------------------------------------------ tree attention
@@ -389,6 +435,8 @@ def test_tree_attention_refuses_what_it_cannot_do():
     with pytest.raises(ValueError, match="memory of its own"):
         wide = torch.zeros(6, 8, 128, dtype=torch.bfloat16, device="cuda")
         ops.rpa_tree_attention(**{**dev, "q": wide[:4]}, out=wide[2:])
+    with pytest.raises(ValueError, match="overlaps an input"):
+        ops.rpa_tree_attention(**dev, out=dev["kv_cache"].view(-1)[: 4 * 8 * 128].view(4, 8, 128))
 
 
 def test_a_captured_step_follows_its_inputs():

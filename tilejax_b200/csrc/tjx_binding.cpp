@@ -157,6 +157,7 @@ PyObject* plan(Args a) {
   Device device;
   for (const at::Tensor* t : in)
     if (t != nullptr) device.add(*t);
+  for (const at::Tensor* t : in) require(t == nullptr || t == in[2] || !overlap(*t, *in[2]), "page_indices overlaps another input");
   const int64_t sizes[6] = {S, S + 1, T, T, S, 2};
   at::Tensor out[6];
   if (a.none(9)) {
@@ -176,6 +177,7 @@ PyObject* plan(Args a) {
       require(is_vector(out[i], sizes[i]), "out is a step of other sizes");
       device.add(out[i]);
       for (const at::Tensor* t : in) require(t == nullptr || !overlap(out[i], *t), "out overlaps an input");
+      for (int j = 0; j < i; ++j) require(!overlap(out[i], out[j]), "out's tensors overlap");
     }
   }
   {
@@ -204,6 +206,28 @@ struct Heads {
       throw BadValue{std::string(name) + "'s last dimension must be dense, its strides multiples of 4 elements, its data 8-byte aligned"};
   }
 };
+// No two elements of an output in one place.
+bool distinct(const at::Tensor& t) {
+  const int64_t tokens = t.size(0), heads = t.size(1), D = t.size(2), token = t.stride(0), head = t.stride(1);
+  auto nested = [D](int64_t n, int64_t inner, int64_t m, int64_t outer) {
+    return (n <= 1 || inner >= D) && (m <= 1 || outer >= (n - 1) * inner + D);
+  };
+  return t.numel() == 0 || nested(heads, head, tokens, token) || nested(tokens, token, heads, head);
+}
+// Two operands without an element in common: apart, or views of one projection's output that share its token stride (side
+// by side within a token, or head by head).
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (!overlap(a, b)) return true;
+  if (a.stride(0) != b.stride(0) || a.stride(0) <= 0) return false;
+  const int64_t difference = (static_cast<int64_t>(address(b)) - static_cast<int64_t>(address(a))) / 2;
+  auto side_by_side = [&](int64_t period, int64_t span_a, int64_t span_b) {
+    const int64_t d = (difference % period + period) % period;
+    return d >= span_a && d + span_b <= period;
+  };
+  const int64_t token = a.stride(0), head = a.stride(1), D = a.size(2);
+  if (side_by_side(token, (a.size(1) - 1) * head + D, (b.size(1) - 1) * b.stride(1) + D)) return true;
+  return head > 0 && b.stride(1) == head && token % head == 0 && side_by_side(head, D, D);
+}
 
 // (q, k, v, q_gamma, k_gamma, positions, cos_sin, kv_cache, slots, eps, interleaved, q_out, k_out) -> (q_out, k_out); v,
 // kv_cache and slots go together.
@@ -246,8 +270,8 @@ PyObject* norm_rope(Args a) {
   } else {
     q_out = a.tensor(11, "out");
     const Heads ho("the queries' output", q_out, T, D);
-    require(ho.heads == H && q_out.device() == device.get() && (same(q_out, q) || !overlap(q_out, q)) &&
-                (same(q_out, q) || (!overlap(q_out, k) && (v == nullptr || !overlap(q_out, *v)))),
+    require(ho.heads == H && q_out.device() == device.get() && (same(q_out, q) || apart(q_out, q)) && apart(q_out, k) &&
+                (v == nullptr || apart(q_out, *v)) && distinct(q_out),
             "the queries' output is q itself or memory of its own, like q");
   }
   strides[6] = q_out.stride(0), strides[7] = q_out.stride(1);
@@ -259,8 +283,8 @@ PyObject* norm_rope(Args a) {
     } else {
       k_out = a.tensor(12, "out");
       const Heads ho("the keys' output", k_out, T, D);
-      require(ho.heads == hk.heads && k_out.device() == device.get() &&
-                  (same(k_out, k) || (!overlap(k_out, q) && !overlap(k_out, k) && !overlap(k_out, q_out))),
+      require(ho.heads == hk.heads && k_out.device() == device.get() && (same(k_out, k) || apart(k_out, k)) &&
+                  apart(k_out, q) && apart(k_out, q_out) && distinct(k_out),
               "the keys' output is k itself or memory of its own, like k");
     }
     strides[8] = k_out.stride(0), strides[9] = k_out.stride(1);
@@ -303,6 +327,8 @@ PyObject* tree_attention(Args a) {
     require(out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.device() == q.device(),
             "out must look like q");
     require(address(out) == address(q) || !overlap(out, q), "out is q itself or memory of its own");
+    for (const at::Tensor* t : {&kv_cache, &kv_lens, &page_indices, &cu_q_lens, &tree_mask, &distribution})
+      require(!overlap(out, *t), "out overlaps an input");
   }
   if (T > 0) {
     const c10::cuda::CUDAGuard guard(device.get());
@@ -334,7 +360,8 @@ PyObject* commit(Args a) {
   } else {
     out = a.tensor(6, "out");
     require(is_vector(out, c.seqs) && out.is_contiguous() && out.device() == device.get(), "out is int32 (S,), on the cache's device");
-    for (const at::Tensor* t : {&kv_lens, &page_indices, &cu_q_lens, &paths, &n_accepted}) require(!overlap(out, *t), "out overlaps an input");
+    for (const at::Tensor* t : {&kv_cache, &kv_lens, &page_indices, &cu_q_lens, &paths, &n_accepted})
+      require(!overlap(out, *t), "out overlaps an input");
   }
   const c10::cuda::CUDAGuard guard(device.get());
   check(commit_fn(kv_cache.data_ptr(), ints(kv_lens), ints(page_indices), ints(cu_q_lens), ints(paths), ints(n_accepted),

@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(PLAN_THREADS, 2) rpa_plan_kernel(const PlanPar
         const int entry = static_cast<int>(page) < of.held
                               ? p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + page]
                               : fresh(of.lack + static_cast<int>(page) - of.held);
-        if (entry >= 0) slot = entry * p.page_size + static_cast<int>(row);
+        const long long at = static_cast<long long>(entry) * p.page_size + row;
+        if (entry >= 0 && at <= 0x7FFFFFFFll) slot = static_cast<int>(at);  // (a table's entry may be anything)
       }
     }
     p.positions[i] = position;
