@@ -643,15 +643,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The larger of three; of a NaN and a number, the number. And the same where a NaN wins.
+// The larger of three; of a NaN and a number, the number. And of two, where a NaN wins.
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 __device__ __forceinline__ float fmax_nan(float a, float b) {

@@ -24,6 +24,12 @@
 // which they join in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
 // the scores), so that the next scores are made while it works, and 128 columns of output.
 //
+// What it reaches: one token a sequence over 64 caches of 1000 to 8100 positions 197 us, 6.0 TB/s of the cache, on pages
+// of 16 as on pages of 128; trees of 16 over 32 caches of up to 4096 64 us; trees of 64 (both row tiles full) over two
+// caches of 125 k 277 us, 0.93 PFLOP/s, and 331 us repeated for a second: then the GPU is at its power limit (1000 W, 1.5 GHz).
+// There a block of 128 positions (whose scores' products read Q from shared memory half as often: 512 cycles for 832, but
+// one score buffer a group) took the same time, repeated and alone, and so did all exponentials on one pipe.
+//
 // A wait tells a barrier's phase from the one before it only. So whoever waits on a ring slot must have seen its use
 // before: rings have an even number of slots and blocks keep their parity over the whole run, so that a group finds
 // its blocks in the same slots always.
@@ -770,8 +776,15 @@ constexpr int TJ_WARPS = 8;
 constexpr int TJ_BATCH = 4;
 
 // The units that several CTAs shared: a CTA per 32 rows (a lane's) joins their partial results in the order of the
-// blocks, a warp 16 of the columns. And the rows that no unit has, which stay the query.
+// blocks, a warp 16 of the columns. And the rows that no unit has, which stay the query (CTAs of the first rows only: the
+// others' exit would wait for the lengths). Bound by latency, a unit's entry and then its parts: 2 us of a call of one
+// sequence, 3 to 5 of larger ones (no launch of it at all: 1 us less than one that returns at once).
 __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
+  int lo = 0, hi = 0;  // the rows that units have (from arrays that were there before either kernel)
+  if (blockIdx.y == 0) {
+    const int seqs = min(max(p.distribution[0], 0), p.S);
+    lo = min(max(p.cu_q_lens[0], 0), p.T), hi = min(max(p.cu_q_lens[seqs], lo), p.T);
+  }
   chain_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = blockIdx.y * 32 + lane;
   const int4 join = p.joins[blockIdx.x];
@@ -812,13 +825,11 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
       dst[k] = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
                           pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
   }
-  if (p.out != p.q) {
-    const int seqs = min(max(p.distribution[0], 0), p.S);
-    const int lo = min(max(p.cu_q_lens[0], 0), p.T), hi = min(max(p.cu_q_lens[seqs], lo), p.T);
+  if (blockIdx.y == 0 && p.out != p.q) {
     const size_t units = static_cast<size_t>(p.H) * TR_D / 8;  // 16 bytes each
     const size_t rest = (static_cast<size_t>(lo) + (p.T - hi)) * units;
-    const size_t step = static_cast<size_t>(gridDim.x) * gridDim.y * TJ_WARPS * 32;
-    for (size_t i = (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * TJ_WARPS * 32 + threadIdx.x; i < rest; i += step) {
+    const size_t step = static_cast<size_t>(gridDim.x) * TJ_WARPS * 32;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * TJ_WARPS * 32 + threadIdx.x; i < rest; i += step) {
       const size_t at = i < lo * units ? i : i + static_cast<size_t>(hi - lo) * units;
       reinterpret_cast<uint4*>(p.out)[at] = reinterpret_cast<const uint4*>(p.q)[at];
     }
