@@ -134,11 +134,16 @@ struct TreePortion {
   int j0, j1;            // blocks of the unit
   bool whole, starts;    // all of the unit's blocks; its first block among them
   bool two;              // two row tiles
-  long long past;        // where the unit's last block starts, seen from the end of the run
+  int past;              // of a unit that ends in a later run: where its last block starts, seen from the end of this one
 };
+// x / weight for x >= 0.
+__device__ __forceinline__ int tree_per_weight(int x, bool two) {
+  return static_cast<int>(two ? static_cast<uint32_t>(x) / TR_COST_TWO : static_cast<uint32_t>(x) / TR_COST_ONE);
+}
 struct TreeWalk {
   int s, hk, pr;
-  long long at, left;  // of the unit's cost, where the walk stands; of the run's, what is left
+  int at;          // of the unit's cost (at most 2^31 / 64 blocks), where the walk stands
+  long long left;  // of the run's, what is left
   TreeSeq q;
   __device__ __forceinline__ void load(const TreeParams& p) {  // by whole warps: the same values, and said to be so
     q = tree_seq(p, s);
@@ -149,16 +154,18 @@ struct TreeWalk {
   __device__ __forceinline__ bool next(const TreeParams& p, TreePortion& o) {
     while (left > 0) {
       const int weight = tree_block_cost(p, q, pr), node0 = pr * 2 * p.tile_nodes;
-      const long long cost = TR_COST_UNIT + static_cast<long long>(q.blocks) * weight, to = at + left;
+      const int cost = TR_COST_UNIT + q.blocks * weight;
+      const bool ends = left >= cost - at;
+      const int to = ends ? cost : at + static_cast<int>(left);
       o.s = s, o.hk = hk, o.ctx = q.ctx, o.end = q.end;
       o.tok = q.tok0 + node0;
       o.nodes = min(q.q_len - node0, 2 * p.tile_nodes);
       o.two = o.nodes > p.tile_nodes;
-      o.j0 = at <= TR_COST_UNIT ? 0 : static_cast<int>(tree_div(at - TR_COST_UNIT + weight - 1, weight));
-      o.j1 = to >= cost ? q.blocks : to <= TR_COST_UNIT ? 0 : static_cast<int>(tree_div(to - TR_COST_UNIT + weight - 1, weight));
+      o.j0 = tree_per_weight(max(at - TR_COST_UNIT, 0) + weight - 1, o.two);
+      o.j1 = ends ? q.blocks : tree_per_weight(max(to - TR_COST_UNIT, 0) + weight - 1, o.two);
       o.starts = o.j0 == 0, o.whole = o.starts && o.j1 == q.blocks;
       o.past = cost - weight - to;
-      left = to - cost, at = 0;
+      left -= cost - at, at = 0;
       if (++pr == q.pairs) {
         pr = 0;
         if (++hk == p.Hkv) {
@@ -463,6 +470,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     const int quarter = warp & 3;   // TMEM lanes of this warp
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;  // of the tile
+    const int node = row / p.group;        // in its tile
     int c = 0, blocks = 0;  // jobs of this group, and blocks of the portions before
     int looked = 0, looked_both = 0, joined = 0;
     bool ok = true;
@@ -481,7 +489,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       const int tile_nodes = u.two ? (tile == 0 ? p.tile_nodes : u.nodes - p.tile_nodes) : u.nodes;
       const int rows = tile_nodes * p.group;
       const bool active = quarter * 32 < rows;  // some row of this warp's is one
-      const int node = row / p.group;           // in its tile
       const bool mine_valid = row < rows;
       const int tok = u.tok + tile * p.tile_nodes + node;
       TreeMask mask;
@@ -757,10 +764,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         ++joined;
         tc_fence_after_sync();
       }
-      if (u.starts && !u.whole && threadIdx.x == 96)
-        p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + 1 + tree_div(u.past, share)));
       blocks += n_blocks;
     }
+    if (ok && blocks > 0 && u.starts && !u.whole && threadIdx.x == 96)  // (the run's last portion)
+      p.joins[blockIdx.x] = make_int4(u.tok, u.nodes, u.hk, static_cast<int>(blockIdx.x + 1 + tree_div(u.past, share)));
   }
 
   tc_fence_before_sync();
