@@ -69,6 +69,7 @@ struct TreeParams {
   int tile_nodes;  // nodes of a row tile: 128 / group
   int box_rows;    // positions of one TMA box: the largest power of two that divides the page size, at most 64
   float scale_log2e;
+  double per_cta;    // 1 / CTAs
   int part_rows;     // rows of a partial result
   float4* part_o;    // [2 CTAs][32][part_rows]: four columns of a row (a warp's rows lie side by side)
   float2* part_ml;   // [2 CTAs][part_rows]: running maximum (log2 units) and sum
@@ -96,9 +97,8 @@ static_assert(TreeSmem::TOTAL <= 232448, "shared memory of one CTA");
 struct TreeSeq {
   int tok0, q_len, ctx, end, blocks, pairs;
 };
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int c0, int c1, int len) {
   TreeSeq r;
-  const int c0 = p.cu_q_lens[s], c1 = p.cu_q_lens[s + 1], len = p.kv_lens[s];
   r.tok0 = min(max(c0, 0), p.T);
   r.q_len = max(min(c1, p.T) - r.tok0, 0);
   r.end = min(max(len, 0), p.pages_per_seq * p.page_size);  // positions to walk
@@ -106,6 +106,10 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
   r.blocks = max((r.end + TR_BLOCK - 1) / TR_BLOCK, 1);     // (one where there is nothing: its rows become zero)
   r.pairs = (r.q_len + 2 * p.tile_nodes - 1) / (2 * p.tile_nodes);
   return r;
+}
+
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
+  return tree_seq(p, p.cu_q_lens[s], p.cu_q_lens[s + 1], p.kv_lens[s]);
 }
 
 // a / b for a >= 0, b > 0: a 64-bit division only where it takes one.
@@ -223,6 +227,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     }
     return;
   }
+  // (Under way while the barriers are set up; without waiting for the number of sequences.)
+  const int per_thread = (p.S + TR_THREADS - 1) / TR_THREADS;
+  const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, p.S), s_hi = min(s_lo + per_thread, p.S);
+  int c0_lo = 0, c1_lo = 0, len_lo = 0;
+  if (s_lo < s_hi) c0_lo = p.cu_q_lens[s_lo], c1_lo = p.cu_q_lens[s_lo + 1], len_lo = p.kv_lens[s_lo];
+  const int distribution = p.distribution[0];
   const uint32_t bar = base + L::BAR_OFF;
   auto q_full = [&](int b) { return bar + 8u * b; };
   auto q_empty = [&](int b) { return bar + 8u * (2 + b); };
@@ -265,16 +275,13 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     tmem_relinquish();
   }
   // All costs added up, and where this CTA's run starts: a thread takes consecutive sequences, the thread that has the
-  // run's first block finds its sequence. (The lengths are read without waiting for the number of sequences.)
+  // run's first block finds its sequence.
   volatile int* start = reinterpret_cast<volatile int*>(base_ptr + L::SCAN_OFF + 96);
-  const int per_thread = (p.S + TR_THREADS - 1) / TR_THREADS;
-  const int s_lo = min(static_cast<int>(threadIdx.x) * per_thread, p.S), s_hi = min(s_lo + per_thread, p.S);
-  const int distribution = p.distribution[0];
   auto cost_of = [&](const TreeSeq& q) { return tree_head_cost(p, q) * p.Hkv; };
   long long mine = 0;
   TreeSeq q_lo{};
   for (int s = s_lo; s < s_hi; ++s) {
-    const TreeSeq q = tree_seq(p, s);
+    const TreeSeq q = s == s_lo ? tree_seq(p, c0_lo, c1_lo, len_lo) : tree_seq(p, s);
     if (s == s_lo) q_lo = q;
     mine += s < distribution ? cost_of(q) : 0;
   }
@@ -287,12 +294,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
   long long total = 0;
-#pragma unroll
-  for (int w = 0; w < TR_THREADS / 32; ++w) {
+  const int scans = min((p.S + 31) / 32, TR_THREADS / 32);  // at least the warps with a sequence
+#pragma unroll 1
+  for (int w = 0; w < scans; ++w) {
     if (w == warp) upto += total;
     total += scan[w];
   }
-  const long long share = max(tree_div(total + gridDim.x - 1, gridDim.x), static_cast<long long>(TR_MIN_SHARE));
+  // (At least total / CTAs, whichever way the product was rounded.)
+  const long long share = max(static_cast<long long>(static_cast<double>(total) * p.per_cta) + 1, static_cast<long long>(TR_MIN_SHARE));
   const long long first = share * blockIdx.x, count = min(share, total - first);  // (count <= 0: nothing)
   if (count > 0 && first >= upto - mine && first < upto) {
     long long off = first - (upto - mine);
@@ -897,6 +906,7 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
   p.status = device_status_word();
   if (p.status == nullptr) return fail(TJX_E_CUDA, "could not locate the device status word");
   const int ctas = sm_count();
+  p.per_cta = 1.0 / ctas;
   p.part_rows = tree_part_rows(T, p.group);
   uint8_t* w = static_cast<uint8_t*>(workspace);
   p.joins = reinterpret_cast<int4*>(w), w += tree_align256(ctas * sizeof(int4));
