@@ -211,8 +211,9 @@ __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
 }
 
-__device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
-  return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
+// Zero times every element, added up: NaN where one is not finite.
+__device__ __forceinline__ void tree_zeros(__nv_bfloat162& sum, uint32_t x) {
+  sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __floats2bfloat162_rn(0.f, 0.f), sum);
 }
 
 __global__ void __launch_bounds__(TR_THREADS, 1)
@@ -544,10 +545,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             m_used = m_new;
             l *= alpha;
             ok = output_done(c - 1);
-            if (!ok) return;
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8 && ok; ++i) {
               uint32_t o[16];
               tmem_ld16(o_tmem + i * 16, o);
               tmem_wait_ld();
@@ -598,14 +598,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         const int v_row = row >> 1, limit = u.end - kv0;
         uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
                                               v_row * 128);
-        bool odd = false;
+        __nv_bfloat162 zeros = __floats2bfloat162_rn(0.f, 0.f);
         if (v_row < limit && v_row >= u.ctx - kv0) {  // (what lies before the nodes every row sees)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint4 x = src[(i + v_row) & 7];  // (eight rows at a time, each at another bank)
-            odd |= not_finite_bf16x2(x.x) || not_finite_bf16x2(x.y) || not_finite_bf16x2(x.z) || not_finite_bf16x2(x.w);
+            tree_zeros(zeros, x.x), tree_zeros(zeros, x.y), tree_zeros(zeros, x.z), tree_zeros(zeros, x.w);
           }
         }
+        const bool odd = __hisnan(zeros.x) || __hisnan(zeros.y);
         uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
         votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
         volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
