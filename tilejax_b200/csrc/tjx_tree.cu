@@ -57,7 +57,7 @@ constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a ga
 // pipeline drained, the rows out. Without the weights the CTA with the most units, or with the widest, ran a third longer
 // than the others (trees of 16 over 32 caches of up to 4096: 81 -> 66 us; of up to 64 over 64 of up to 8100: 340 -> 311).
 constexpr int TR_COST_ONE = 4, TR_COST_TWO = 6, TR_COST_UNIT = 32;
-constexpr int TR_MIN_SHARE = 12;  // a run's cost, at least (it may not be shorter than a block)
+constexpr int TR_MIN_SHARE = 8;  // a run's cost, at least: two blocks of one row tile, one a group (one sequence 11.8 us with 12, 11.0; 11.5 with 6)
 static_assert(TR_MIN_SHARE >= TR_COST_TWO && TR_MIN_SHARE >= TR_COST_ONE, "every run inside a unit has a block");
 
 struct TreeParams {
