@@ -24,11 +24,13 @@
 // which they join in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
 // the scores), so that the next scores are made while it works, and 128 columns of output.
 //
-// What it reaches: one token a sequence over 64 caches of 1000 to 8100 positions 197 us, 6.0 TB/s of the cache, on pages
-// of 16 as on pages of 128; trees of 16 over 32 caches of up to 4096 64 us; trees of 64 (both row tiles full) over two
-// caches of 125 k 277 us, 0.93 PFLOP/s, and 331 us repeated for a second: then the GPU is at its power limit (1000 W, 1.5 GHz).
-// There a block of 128 positions (whose scores' products read Q from shared memory half as often: 512 cycles for 832, but
-// one score buffer a group) took the same time, repeated and alone, and so did all exponentials on one pipe.
+// What it reaches: one token a sequence over 64 caches of 1000 to 8100 positions 194 us, 6.1 TB/s of the cache, on pages
+// of 16 as on pages of 128; trees of 16 over 32 caches of up to 4096 62 us; trees of 64 (both row tiles full) over two
+// caches of 125 k 265 us, 0.97 PFLOP/s, and 318 us repeated for a second: then the GPU is at its power limit (1000 W, 1.5 GHz).
+// There blocks of 128 positions (whose scores' products read Q from shared memory half as often: 512 cycles for 832, but
+// one score buffer a group) took the same time, repeated and alone, and so did all exponentials on one pipe. What a unit
+// takes beside its blocks is to a large part code that is not in the instruction cache when its turn comes: less of it (104 to
+// 89 KB) made every call shorter, by 3 to 5 %.
 //
 // A wait tells a barrier's phase from the one before it only. So whoever waits on a ring slot must have seen its use
 // before: rings have an even number of slots and blocks keep their parity over the whole run, so that a group finds
@@ -54,8 +56,8 @@ constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a r
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
 // What a run is cut by, in units of about 300 cycles: a block of one row tile (bound by its loads, 1230 cycles), of two
 // (by their softmax, 1950), and what a unit takes beside its blocks: the last scores masked and their V rows looked at, the
-// pipeline drained, the rows out. Without the weights the CTA with the most units, or with the widest, ran a third longer
-// than the others (trees of 16 over 32 caches of up to 4096: 81 -> 66 us; of up to 64 over 64 of up to 8100: 340 -> 311).
+// pipeline drained, the rows out. Without the weights the CTA with the most units, or with the widest, runs longer
+// than the others (trees of 16 over 32 caches of up to 4096: 69.5 -> 61.5 us; of up to 64 over 64 of up to 8100: 325 -> 289).
 constexpr int TR_COST_ONE = 4, TR_COST_TWO = 6, TR_COST_UNIT = 32;
 constexpr int TR_MIN_SHARE = 8;  // a run's cost, at least: two blocks of one row tile, one a group (one sequence 11.8 us with 12, 11.0; 11.5 with 6)
 static_assert(TR_MIN_SHARE >= TR_COST_TWO && TR_MIN_SHARE >= TR_COST_ONE, "every run inside a unit has a block");
