@@ -387,6 +387,18 @@ def test_scores_hundreds_apart(rising):
     check_tree(inp, slack=2.0**-5)
 
 
+def test_the_next_sequences_queries_do_not_change_a_bit():
+    # They fill the rest of a row tile, and a raised maximum is raised for a whole warp. Large ones raise it in most blocks.
+    inp = tree_case([9, 13, 3], [1500, 1500, 700], 16, 2, 16, poison=False)
+    dev = {k: to_device(v) for k, v in inp.items()}
+    want = ops.rpa_tree_attention(**dev, sm_scale=128**-0.5)
+    for first in (9, 22):
+        louder = dev["q"].clone()
+        louder[first:] *= 32
+        got = ops.rpa_tree_attention(**{**dev, "q": louder}, sm_scale=128**-0.5)
+        assert torch.equal(got[:first], want[:first]) and not torch.equal(got[first:], want[first:])
+
+
 def test_a_longer_tree_than_its_cache_and_lengths_past_the_table():
     inp = tree_case([6, 4], [20, 30], 8, 2, 16)
     inp["kv_lens"][0] = 4          # four positions for six nodes: the first two are in no cache row

@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           if (m_blk == INFINITY) m_blk = NAN;
           if (last_job < 0) {
             m_used = fmax_nan(m_blk, TR_NOTHING);
-          } else if (__builtin_expect(__any_sync(0xFFFFFFFFu, !(m_blk <= m_used + TR_RESCALE)), 0)) {
+          } else if (__builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && !(m_blk <= m_used + TR_RESCALE)), 0)) {
+            // (Rows of the tile that are none hold other sequences' queries, in place even while those change: they have no say.)
             const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
