@@ -311,11 +311,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     int s = s_lo;
     TreeSeq q = q_lo;
     for (long long n; off >= (n = cost_of(q)); q = tree_seq(p, ++s)) off -= n;
-    const int hk = static_cast<int>(tree_div(off, tree_head_cost(p, q)));
-    off -= hk * tree_head_cost(p, q);
-    const int pr = static_cast<int>(min(tree_div(off, tree_pair_cost(q)), static_cast<long long>(q.pairs - 1)));
-    start[0] = s, start[1] = hk, start[2] = pr, start[3] = static_cast<int>(off - pr * tree_pair_cost(q));
-    start[4] = q.tok0, start[5] = q.q_len, start[6] = q.ctx, start[7] = q.end, start[8] = q.blocks, start[9] = q.pairs;
+    start[0] = s, start[1] = q.tok0, start[2] = q.q_len, start[3] = q.ctx, start[4] = q.end, start[5] = q.blocks;
+    start[6] = q.pairs, start[7] = static_cast<int>(off), start[8] = static_cast<int>(off >> 32);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -325,11 +322,21 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   // loop counters per lane.)
   TreeWalk walk;
   {
-    const int word = lane < 10 ? start[lane] : 0;
+    const int word = lane < 9 ? start[lane] : 0;
     auto get = [&](int i) { return __shfl_sync(0xFFFFFFFFu, word, i); };
-    walk.s = get(0), walk.hk = get(1), walk.pr = get(2), walk.at = get(3);
-    walk.q.tok0 = get(4), walk.q.q_len = get(5), walk.q.ctx = get(6), walk.q.end = get(7), walk.q.blocks = get(8);
-    walk.q.pairs = get(9), walk.left = __shfl_sync(0xFFFFFFFFu, count, 0);
+    walk.s = get(0), walk.hk = 0, walk.pr = 0, walk.at = 0, walk.left = __shfl_sync(0xFFFFFFFFu, count, 0);
+    walk.q.tok0 = get(1), walk.q.q_len = get(2), walk.q.ctx = get(3), walk.q.end = get(4), walk.q.blocks = get(5);
+    walk.q.pairs = get(6);
+    long long off = static_cast<long long>(static_cast<uint32_t>(get(7))) | (static_cast<long long>(get(8)) << 32);
+    if (walk.left > 0) {  // (else nothing was found)
+      // The KV head, and the unit of it: counted by the lanes, 32 at a time, each of which costs the same.
+      const long long head = tree_head_cost(p, walk.q), pair = tree_pair_cost(walk.q);
+      for (int n = 32; n == 32; walk.hk += n) n = __popc(__ballot_sync(0xFFFFFFFFu, (walk.hk + lane + 1) * head <= off));
+      off -= walk.hk * head;
+      for (int n = 32; n == 32; walk.pr += n)
+        n = __popc(__ballot_sync(0xFFFFFFFFu, walk.pr + lane + 1 < walk.q.pairs && (walk.pr + lane + 1) * pair <= off));
+      walk.at = static_cast<int>(off - walk.pr * pair);
+    }
   }
 
   if (warp == 0 || warp == 11) {
