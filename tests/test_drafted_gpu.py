@@ -433,6 +433,63 @@ def test_nan_in_a_hidden_node_stays_there():
         assert np.isnan(got[~blind][..., :64]).all() and np.isposinf(got[~blind][..., 64:]).all()
 
 
+def check_tree_not_finite(inp, sm_scale=128**-0.5):
+    """As check_tree, where some elements are NaN by the formula: the same ones, and the others as close as ever."""
+    got = f64(to_host(ops.rpa_tree_attention(**{k: to_device(v) for k, v in inp.items()}, sm_scale=sm_scale)))
+    with np.errstate(invalid="ignore"):
+        want, size = oracle.tree_attention_f64(*inp.values(), sm_scale)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    close(got[fine], want[fine], size[fine], 2.0**-8 + 2.0**-11)
+    return want
+
+
+SCORE_CASES = {  # (nodes, ctx, heads): every head has KV head 0, pages of 16
+    "one masked block": (5, 20, 4),
+    "whole blocks before": (6, 300, 4),
+    "two row tiles": (40, 330, 8),
+    "split": (4, 9000, 4),
+}
+
+
+@pytest.mark.parametrize("kind", ["all minus", "all minus but one", "all minus at first", "plus", "nan", "one key minus", "hidden"])
+@pytest.mark.parametrize("name", SCORE_CASES)
+def test_scores_that_are_not_finite(name, kind):
+    # An infinite query element meets keys of one sign: a row whose scores are all minus infinity is NaN (0 / 0), not a mean
+    # of some values; one that sees a single finite score is that position's value.
+    nodes, ctx, heads = SCORE_CASES[name]
+    inp = tree_case([nodes], [ctx + nodes], heads, 1, 16, seed=ctx)
+    table = inp["page_indices"]
+    keys = [inp["kv_cache"][table[p // 16], p % 16, 0, 0] for p in range(ctx + nodes)]  # views, (128,) each
+    q, node = inp["q"], min(2, nodes - 1)
+    if kind.startswith("all minus"):
+        q[node, :2, 7] = np.inf
+        for k in keys:
+            k[7] = -abs(k[7].astype(np.float32)) - 1
+        if kind.endswith("one"):
+            keys[ctx // 2][7] = 0          # 0 * inf: NaN
+            q[node, 1] = -np.inf           # and a row whose every element is infinite
+        if kind.endswith("first"):         # finite scores from the middle on
+            q[..., 7], q[node, :2, 7] = -1.0, -3e38
+            for k in keys[: ctx // 2]:
+                k[:] = 0
+                k[7] = np.inf
+            for k in keys[ctx // 2 :]:
+                k[7] = 0
+    elif kind == "plus":
+        keys[ctx // 2][5], q[node, 1, 5] = np.inf, 1.0
+        q[node, 2, 5] = -1.0
+    elif kind == "nan":
+        q[node, 3, 9] = np.nan
+    elif kind == "one key minus":          # a position of weight zero for every row
+        keys[ctx - 3][5], q[:, :, 5] = -np.inf, 1.0
+    else:                                  # a hidden node's key: rows that do not see it are as without it
+        keys[ctx + 1][:] = np.nan
+    want = check_tree_not_finite(inp)
+    assert np.isnan(want).any() == (kind not in ("all minus at first", "one key minus"))
+    assert np.isfinite(want).any()
+
+
 def test_tree_attention_refuses_what_it_cannot_do():
     dev = {k: to_device(v) for k, v in tree_case([4], [40], 8, 2, 16).items()}
     for scale in (0.0, -1.0, float("nan"), float("inf")):

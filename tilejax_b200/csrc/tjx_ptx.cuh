@@ -658,7 +658,7 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
 // 2^x for a pair of elements. POLY: on the FMA pipe — x = n + f with n the nearest integer (the float trick of
 // adding 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f by a cubic fitted to a relative error of 7.5e-5 (P is rounded to
 // bf16, 3.9e-3, right after); n goes into the exponent field by integer addition. x below -125 is held there
-// (2^-125: nothing, after the rounding of P V and of the row sum).
+// (2^-125: nothing, after the rounding of P V and of the row sum, beside any weight that counts; minus infinity too).
 __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {  // `poly` is a constant after unrolling
   if (!poly) {
     return make_float2(ex2(x.x), ex2(x.y));

@@ -52,7 +52,9 @@ constexpr int TR_K_STAGES = 4;
 constexpr int TR_V_STAGES = 6;  // a V block is held longer: until its probabilities are made
 constexpr int TR_THREADS = 384;
 constexpr float TR_LOG2E = 1.4426950408889634f;
-constexpr float TR_NOTHING = -1e30f;  // the running maximum (log2 units) of a row that has seen nothing
+// The running maximum (log2 units) of a row that has seen no score above minus infinity: the lowest number, so that no score
+// is below it. Its sum tells whether it has seen one at all: 0 if not, else something.
+constexpr float TR_NOTHING = -3.402823466e38f;
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
 // What a run is cut by, in units of about 300 cycles: a block of one row tile (bound by its loads, 1230 cycles), of two
 // (by their softmax, 1950), and what a unit takes beside its blocks: the last scores masked and their V rows looked at, the
@@ -211,6 +213,11 @@ __device__ __forceinline__ uint32_t tree_bits(const TreeMask& mask, int pos, int
 __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   if (__builtin_expect(__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity) != 0), 1)) return true;
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
+}
+
+// What a row's products are weighed by: zero where it sees nothing, NaN where it sees minus infinity only (0 / 0 by the formula).
+__device__ __forceinline__ float tree_inverse(float m, float sum) {
+  return sum == 0.f ? 0.f : m == TR_NOTHING ? NAN : 1.0f / sum;
 }
 
 // Zero times every element, added up: NaN where one is not finite.
@@ -518,8 +525,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       float m_used = TR_NOTHING, l = 0.f;
       int last_job = -1;
       // Job c: its scores out of TMEM, its weights into it over them. `see0`, `see1`: the positions this row sees, where
-      // `masked`. A score that is NaN or infinite makes the row NaN, as the formula does: through the maximum, since not
-      // every way to an exponential keeps a NaN.
+      // `masked`. A score that is NaN or plus infinity makes the row NaN, as the formula does: through the maximum, since not
+      // every way to an exponential keeps a NaN. Minus infinity weighs nothing beside a larger score and makes a row NaN
+      // that has no other (tree_inverse).
       auto job = [&](auto masked, int block, uint32_t see0, uint32_t see1, uint32_t (&pk)[32]) {
         ok = wait(s_full(t, c & 1), (c >> 1) & 1, TJX_ERR_WAIT_TMEM_FULL);
         if (!ok) return;
@@ -569,7 +577,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           }
           // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention); the
           // sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA pipe, but
-          // where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0).
+          // where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0, one that sees minus
+          // infinity only has 1 instead; without hidden positions it has what the FMA pipe's exponentials are held at).
           const float2 scale = make_float2(p.scale_log2e, p.scale_log2e), neg_m = make_float2(-m_used, -m_used);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -582,6 +591,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
               pk[h * 16 + (i >> 1)] = pack_bf16(e.x, e.y);
             }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          if (masked.value && m_used == TR_NOTHING && (see0 | see1) != 0) l = 1.f;
           tmem_st32(s_tmem, pk);
           tmem_wait_st();
         }
@@ -726,7 +736,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       const size_t ml_row = static_cast<size_t>(part) * p.part_rows + tile * p.tile_nodes * p.group + row;
       if (u.two) {
         tc_fence_after_sync();
-        const float inv = u.whole ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
+        const float inv = u.whole ? tree_inverse(m_used, l) : 1.0f;
         if (active) {
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
@@ -758,7 +768,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           float w0 = ex2(a.x - m), w1 = ex2(b.x - m);
           const float sum = a.y * w0 + b.y * w1;
           if (u.whole) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            const float inv = tree_inverse(m, sum);
             w0 *= inv, w1 *= inv;
           }
 #pragma unroll 1
@@ -844,7 +854,7 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
         }
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const float inv = tree_inverse(m, sum);
     const size_t row = static_cast<size_t>(join.x + x / p.group) * p.H + join.z * p.group + x % p.group;
     uint4* dst = reinterpret_cast<uint4*>(p.out + row * TR_D + 16 * warp);
 #pragma unroll
