@@ -490,6 +490,22 @@ def test_scores_that_are_not_finite(name, kind):
     assert np.isfinite(want).any()
 
 
+@pytest.mark.parametrize("sm_scale", [1e4, 1e10, 1e30])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("name", SCORE_CASES)
+def test_scores_near_the_ends_of_the_range(name, sign, sm_scale):
+    # One channel makes the scores, so f32 has them exactly, and they are whole: two of them are the same or so far apart that
+    # the smaller has no weight. The row is the mean of V over its largest scores, whatever their size.
+    nodes, ctx, heads = SCORE_CASES[name]
+    inp = tree_case([nodes], [ctx + nodes], heads, 1, 16, seed=ctx)
+    rng = np.random.default_rng(ctx)
+    inp["q"][:] = 0
+    inp["q"][..., 3] = sign
+    for p in range(ctx + nodes):
+        inp["kv_cache"][inp["page_indices"][p // 16], p % 16, 0, 0, 3] = 1 + rng.integers(0, 200)
+    check_tree(inp, sm_scale)
+
+
 def test_tree_attention_refuses_what_it_cannot_do():
     dev = {k: to_device(v) for k, v in tree_case([4], [40], 8, 2, 16).items()}
     for scale in (0.0, -1.0, float("nan"), float("inf")):

@@ -55,6 +55,10 @@ constexpr float TR_LOG2E = 1.4426950408889634f;
 // The running maximum (log2 units) of a row that has seen no score above minus infinity: the lowest number, so that no score
 // is below it. Its sum tells whether it has seen one at all: 0 if not, else something.
 constexpr float TR_NOTHING = -3.402823466e38f;
+// From this maximum on (log2 units) a row's scores are rounded before the maximum is taken off. Below it that is one fused
+// step, which is more exact but leaves the maximum's own rounding in every exponent (at most 8 here): the same for all of the
+// row, so gone after the division by the sum, unless it leaves f32's range, as it would from some 2^31 on.
+constexpr float TR_FAR = 268435456.f;
 constexpr float TR_RESCALE = 8.0f;    // raise the running maximum only for a gain of 2^8: the same result, rarely a rescale
 // What a run is cut by, in units of about 300 cycles: a block of one row tile (bound by its loads, 1230 cycles), of two
 // (by their softmax, 1950), and what a unit takes beside its blocks: the last scores masked and their V rows looked at, the
@@ -555,10 +559,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int i = 0; i < 32; ++i) mx[i & 3] = fmax_nan(mx[i & 3], __uint_as_float(v[h][i]));
           float m_blk = fmax_nan(fmax_nan(mx[0], mx[1]), fmax_nan(mx[2], mx[3])) * p.scale_log2e;
           if (m_blk == INFINITY) m_blk = NAN;
-          if (last_job < 0) {
-            m_used = fmax_nan(m_blk, TR_NOTHING);
-          } else if (__builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && !(m_blk <= m_used + TR_RESCALE)), 0)) {
-            // (Rows of the tile that are none hold other sequences' queries, in place even while those change: they have no say.)
+          if (last_job < 0) m_used = fmax_nan(m_blk, TR_NOTHING);
+          float scale_log2e = p.scale_log2e;
+          // (Rows of the tile that are none hold other sequences' queries, in place even while those change: they have no say.)
+          const bool raise = !(m_blk <= m_used + TR_RESCALE), far = fabsf(m_blk) >= TR_FAR && m_blk != -INFINITY;
+          if (__builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && far), 0)) {
+            const float factor = far ? scale_log2e : 1.f;
+            scale_log2e = far ? 1.f : scale_log2e;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) * factor);
+          }
+          if (last_job >= 0 && __builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && raise), 0)) {
             const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
@@ -579,7 +592,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           // sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA pipe, but
           // where positions are hidden: there zero must be zero (a row that sees nothing has the sum 0, one that sees minus
           // infinity only has 1 instead; without hidden positions it has what the FMA pipe's exponentials are held at).
-          const float2 scale = make_float2(p.scale_log2e, p.scale_log2e), neg_m = make_float2(-m_used, -m_used);
+          const float2 scale = make_float2(scale_log2e, scale_log2e), neg_m = make_float2(-m_used, -m_used);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int h = 0; h < 2; ++h)
