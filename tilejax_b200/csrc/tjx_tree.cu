@@ -219,6 +219,8 @@ __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code)) != 0;
 }
 
+__device__ __forceinline__ bool tree_far(float m) { return fabsf(m) >= TR_FAR && m != TR_NOTHING; }
+
 // What a row's products are weighed by: zero where it sees nothing, NaN where it sees minus infinity only (0 / 0 by the formula).
 __device__ __forceinline__ float tree_inverse(float m, float sum) {
   return sum == 0.f ? 0.f : m == TR_NOTHING ? NAN : 1.0f / sum;
@@ -527,6 +529,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       mask.second = mask.words > 1 ? static_cast<uint32_t>(mask.row[1]) : 0u;
       const uint32_t o_tmem = tmem_base + lane_addr + 256 + t * 128;
       float m_used = TR_NOTHING, l = 0.f;
+      bool far = false;    // some row's maximum is far from zero
+      bool again = false;  // the first loop has left a block to the second, its scores read
       int last_job = -1;
       // Job c: its scores out of TMEM, its weights into it over them. `see0`, `see1`: the positions this row sees, where
       // `masked`. A score that is NaN or plus infinity makes the row NaN, as the formula does: through the maximum, since not
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (!ok) return;
         tc_fence_after_sync();
         // The scores are there, so the block's keys have been read. (An arrival here is cheaper than the issuer's commit.)
-        if (quarter == 0 && lane == 0) mbar_arrive(k_empty((blocks + block) % TR_K_STAGES));
+        if (quarter == 0 && lane == 0 && !again) mbar_arrive(k_empty((blocks + block) % TR_K_STAGES));
         if (active) {
           const uint32_t s_tmem = tmem_base + lane_addr + t * 128 + (c & 1) * 64;
           uint32_t v[2][32];
@@ -559,34 +563,40 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int i = 0; i < 32; ++i) mx[i & 3] = fmax_nan(mx[i & 3], __uint_as_float(v[h][i]));
           float m_blk = fmax_nan(fmax_nan(mx[0], mx[1]), fmax_nan(mx[2], mx[3])) * p.scale_log2e;
           if (m_blk == INFINITY) m_blk = NAN;
-          if (last_job < 0) m_used = fmax_nan(m_blk, TR_NOTHING);
-          float scale_log2e = p.scale_log2e;
           // (Rows of the tile that are none hold other sequences' queries, in place even while those change: they have no say.)
-          const bool raise = !(m_blk <= m_used + TR_RESCALE), far = fabsf(m_blk) >= TR_FAR && m_blk != -INFINITY;
-          if (__builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && far), 0)) {
-            const float factor = far ? scale_log2e : 1.f;
-            scale_log2e = far ? 1.f : scale_log2e;
+          if (last_job < 0 || __builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && !(m_blk <= m_used + TR_RESCALE)), 0)) {
+            const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
+            if (!far && __any_sync(0xFFFFFFFFu, mine_valid && tree_far(m_new))) {
+              far = true;
+              again = !masked.value;
+              if (again) return;
+            }
+            m_used = m_new;
+            if (last_job >= 0) {
+              l *= alpha;
+              ok = output_done(c - 1);
+              tc_fence_after_sync();
+#pragma unroll 1
+              for (int i = 0; i < 8 && ok; ++i) {
+                uint32_t o[16];
+                tmem_ld16(o_tmem + i * 16, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                tmem_st16(o_tmem + i * 16, o);
+              }
+              tmem_wait_st();
+            }
+          }
+          float scale_log2e = p.scale_log2e;
+          if (masked.value && __builtin_expect(far, 0)) {
+            const bool mine = tree_far(m_used);
+            const float factor = mine ? scale_log2e : 1.f;
+            scale_log2e = mine ? 1.f : scale_log2e;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(__uint_as_float(v[h][i]) * factor);
-          }
-          if (last_job >= 0 && __builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && raise), 0)) {
-            const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
-            m_used = m_new;
-            l *= alpha;
-            ok = output_done(c - 1);
-            tc_fence_after_sync();
-#pragma unroll 1
-            for (int i = 0; i < 8 && ok; ++i) {
-              uint32_t o[16];
-              tmem_ld16(o_tmem + i * 16, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-              tmem_st16(o_tmem + i * 16, o);
-            }
-            tmem_wait_st();
           }
           // P is rounded to bf16 for the tensor cores (off by 2^-8 of itself, as in the framework's other attention); the
           // sum adds the unrounded values. Two elements an instruction; a quarter of the exponentials on the FMA pipe, but
@@ -615,52 +625,57 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       };
       int block = u.two ? 0 : (t - blocks) & 1;
       const int step = u.two ? 1 : 2;
-      // Blocks that every row sees whole.
+      // Blocks that every row sees whole, while no maximum is far from zero (the second loop rounds such scores: 64 products more,
+      // whose code in this one would cost more than they do).
       const int plain = min(max(min(u.ctx, u.end) / TR_BLOCK - u.j0, 0), n_blocks);
       for (; block < plain && ok; block += step, ++c) {
         uint32_t pk[32];
         job(std::false_type{}, block, 0u, 0u, pk);
+        if (again) break;
       }
       // Blocks with positions that some row does not see, or that are none. What a row does not see must not reach it: zero
       // times NaN is NaN. So rows of V past the end are zeroed, and rows holding anything but finite numbers too, which are
       // then added by hand to the rows that see them.
       for (; block < n_blocks && ok; block += step, ++c) {
         const int kv0 = (u.j0 + block) * TR_BLOCK, stage = (blocks + block) % TR_V_STAGES;
-        ok = wait(v_full(stage), ((blocks + block) / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
-        if (!ok) break;
-        const int v_row = row >> 1, limit = u.end - kv0;
-        uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
-                                              v_row * 128);
-        __nv_bfloat162 zeros = __floats2bfloat162_rn(0.f, 0.f);
-        if (v_row < limit && v_row >= u.ctx - kv0) {  // (what lies before the nodes every row sees)
+        uint32_t bad[4] = {};
+        if (block >= plain) {
+          ok = wait(v_full(stage), ((blocks + block) / TR_V_STAGES) & 1, TJX_ERR_WAIT_FULL);
+          if (!ok) break;
+          const int v_row = row >> 1, limit = u.end - kv0;
+          uint4* src = reinterpret_cast<uint4*>(base_ptr + L::V_OFF + stage * L::KV_BYTES + (row & 1) * (L::KV_BYTES / 2) +
+                                                v_row * 128);
+          __nv_bfloat162 zeros = __floats2bfloat162_rn(0.f, 0.f);
+          if (v_row < limit && v_row >= u.ctx - kv0) {  // (what lies before the nodes every row sees)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 x = src[(i + v_row) & 7];  // (eight rows at a time, each at another bank)
-            tree_zeros(zeros, x.x), tree_zeros(zeros, x.y), tree_zeros(zeros, x.z), tree_zeros(zeros, x.w);
+            for (int i = 0; i < 8; ++i) {
+              const uint4 x = src[(i + v_row) & 7];  // (eight rows at a time, each at another bank)
+              tree_zeros(zeros, x.x), tree_zeros(zeros, x.y), tree_zeros(zeros, x.z), tree_zeros(zeros, x.w);
+            }
           }
-        }
-        const bool odd = __hisnan(zeros.x) || __hisnan(zeros.y);
-        uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
-        votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
-        volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
-        if (lane == 0) {
-          flags[quarter] = votes;
-          mbar_arrive(u.two ? v_seen_both : v_seen(t));
-        }
-        ok = u.two ? wait(v_seen_both, looked_both & 1, TJX_ERR_WAIT_OTHER) : wait(v_seen(t), looked & 1, TJX_ERR_WAIT_OTHER);
-        if (u.two) ++looked_both; else ++looked;
-        if (!ok) break;
-        uint32_t bad[4];
+          const bool odd = __hisnan(zeros.x) || __hisnan(zeros.y);
+          uint32_t votes = __ballot_sync(0xFFFFFFFFu, odd);
+          votes = (votes | (votes >> 1)) & 0x55555555u;  // bit 2 i: row i of this warp's sixteen
+          volatile uint32_t* flags = bad_rows + (t * 2 + (c & 1)) * 4;
+          if (lane == 0) {
+            flags[quarter] = votes;
+            mbar_arrive(u.two ? v_seen_both : v_seen(t));
+          }
+          ok = u.two ? wait(v_seen_both, looked_both & 1, TJX_ERR_WAIT_OTHER) : wait(v_seen(t), looked & 1, TJX_ERR_WAIT_OTHER);
+          if (u.two) ++looked_both; else ++looked;
+          if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad[i] = flags[i];
-        if (v_row >= limit || ((flags[v_row >> 4] >> (2 * (v_row & 15))) & 1)) {
+          for (int i = 0; i < 4; ++i) bad[i] = flags[i];
+          if (v_row >= limit || ((flags[v_row >> 4] >> (2 * (v_row & 15))) & 1)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) src[(i + v_row) & 7] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8; ++i) src[(i + v_row) & 7] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
         const uint32_t see0 = tree_bits(mask, kv0, u.ctx, u.end), see1 = tree_bits(mask, kv0 + 32, u.ctx, u.end);
         uint32_t pk[32];
         job(std::true_type{}, block, see0, see1, pk);
+        again = false;
         if (ok && active && (bad[0] | bad[1] | bad[2] | bad[3]) != 0) {
           // The rows of V that were taken out, once this block's product is in.
           ok = output_done(c);
