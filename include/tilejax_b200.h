@@ -297,6 +297,9 @@ int tjx_ragged_paged_attention_bf16(const void* q, const void* keys, const void*
  *   positions[t] = ctx_lens[s] + the token's index in its sequence, or ctx_lens[s] + depths[t] where depths is given (a
  *                drafted token's depth in its tree); slots[t] = its page * page_size + its row of the page, -1 where it
  *                has no page (none left, or past the table). Rows behind the last token: position 0, slot -1.
+ * kv_lens counts tokens without a page too: nothing is written for them, and tjx_rpa_tree_attention_bf16 has no row see
+ * them. A caller that goes on with such a sequence (n_free_out[1] > 0; pages_held_out[s] * page_size < kv_lens[s]) brings
+ * those tokens again, or leaves it out of the step's decode and prefill.
  * free_capacity is the length of free_pages. No output may overlap an input (NULL aside). At most 8192 sequences. */
 int tjx_rpa_plan(const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* pages_held, const int32_t* depths,
                  int32_t* page_indices, const int32_t* free_pages, const int32_t* n_free, int free_capacity, int S, int T,
@@ -325,8 +328,9 @@ size_t tjx_rpa_tree_attention_workspace_bytes(int T, int S, int H, int Hkv);
  * s < distribution[0] has q_len = cu_q_lens[s + 1] - cu_q_lens[s] new tokens ("nodes"), node j at cache position
  * kv_lens[s] - q_len + j (already written). Each attends, scores times sm_scale, to every position before those and to
  * the nodes j whose bit (bit j % 32 of word j / 32) is set in its row of tree_mask int32[T, words]; a node past the
- * words is seen by none. A row that sees nothing is zero; what hidden positions hold, NaN included, does not reach the
- * result. Every other row of out [T, H, D] is q's (out may be q), as after tjx_rpa_decode_bf16: tjx_rpa_prefill_bf16
+ * words is seen by none, and so is a position whose entry of page_indices is no page of the cache, as tjx_rpa_plan's -1
+ * (tjx_rpa_decode_bf16 and tjx_rpa_prefill_bf16 clamp such an entry, as the reference's gather does). A row that sees
+ * nothing is zero; what hidden positions hold, NaN included, does not reach the result. Every other row of out [T, H, D] is q's (out may be q), as after tjx_rpa_decode_bf16: tjx_rpa_prefill_bf16
  * with out as its q then serves the sequences from distribution[0] on.
  *   workspace: at least tjx_rpa_tree_attention_workspace_bytes(...) bytes, 256-byte aligned
  * Constraints: D == 128; H a multiple of Hkv, H / Hkv <= 128; page_size a multiple of 16; sm_scale > 0. */

@@ -73,7 +73,8 @@ def pack_tree_mask(sees, words=None):
 
 def tree_attention_f64(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution, sm_scale):
     """(the rows in float64, the mean of |v| under each row's weights: what the weights' rounding is relative to). Rows no
-    sequence below distribution[0] has are q's. Positions a row does not see are left out, whatever they hold."""
+    sequence below distribution[0] has are q's. Positions a row does not see are left out, whatever they hold, and so are those
+    whose table entry is no page of the cache."""
     pages, page_size, hkv, _, D = kv_cache.shape
     T, H, _ = q.shape
     S = len(kv_lens)
@@ -86,11 +87,13 @@ def tree_attention_f64(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask,
         t0, t1 = int(cu_q_lens[s]), int(cu_q_lens[s + 1])
         length = min(max(int(kv_lens[s]), 0), table.shape[1] * page_size)
         ctx = int(kv_lens[s]) - (t1 - t0)
-        where = np.clip(table[s, np.arange(length) // page_size], 0, pages - 1)
+        entry = table[s, np.arange(length) // page_size]
+        paged = (entry >= 0) & (entry < pages)
+        where = np.where(paged, entry, 0)
         rows = np.asarray(kv_cache)[where, np.arange(length) % page_size].astype(np.float64)  # (length, hkv, 2, D)
         for t in range(t0, t1):
-            sees = [p for p in range(length) if p < ctx or
-                    (p - ctx < 32 * bits.shape[1] and (int(bits[t, (p - ctx) // 32]) >> ((p - ctx) % 32)) & 1)]
+            sees = [p for p in range(length) if paged[p] and (p < ctx or
+                    (p - ctx < 32 * bits.shape[1] and (int(bits[t, (p - ctx) // 32]) >> ((p - ctx) % 32)) & 1))]
             if not sees:
                 out[t] = 0
                 continue

@@ -506,6 +506,28 @@ def test_scores_near_the_ends_of_the_range(name, sign, sm_scale):
     check_tree(inp, sm_scale)
 
 
+@pytest.mark.parametrize("where", ["end", "middle", "first", "all"])
+@pytest.mark.parametrize("name", ["ragged", "a page inside", "two row tiles", "many rows", "split", "one token, long"])
+def test_positions_without_a_page_are_seen_by_none(name, where):
+    # Entries that are no page of the pool, as rpa_plan leaves them where the stack ran out: neither a stand-in page nor NaN
+    # in one reaches the result, and a row that sees nothing else is zero.
+    q_lens, kv_lens, heads, kv_heads, page = TREES[name]
+    inp = tree_case(q_lens, kv_lens, heads, kv_heads, page, seed=5)
+    pool = len(inp["kv_cache"])
+    table = inp["page_indices"].reshape(len(q_lens), -1)
+    for s, n in enumerate(kv_lens):
+        used = -(-n // page)
+        gone = {"end": range(used - (used + 2) // 3, used), "middle": range(used // 3, used // 2 + 1), "first": [0],
+                "all": range(used)}[where]
+        for i, entry in enumerate(gone):
+            table[s, entry] = [-1, pool, 2**31 - 1, -(2**31)][i % 4]
+    for stand_in in (0, pool - 1):
+        if stand_in not in table:
+            inp["kv_cache"][stand_in] = np.nan
+    got = check_tree(inp)
+    assert where != "all" or not got.any()
+
+
 def test_tree_attention_refuses_what_it_cannot_do():
     dev = {k: to_device(v) for k, v in tree_case([4], [40], 8, 2, 16).items()}
     for scale in (0.0, -1.0, float("nan"), float("inf")):

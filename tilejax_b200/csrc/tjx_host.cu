@@ -110,7 +110,7 @@ static EncodeTiledFn encode_fn() {
 
 int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int elem_bytes, int rank,
                     const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                    CUtensorMapSwizzle swizzle) {
+                    CUtensorMapSwizzle swizzle, CUtensorMapFloatOOBfill behind) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(TJX_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) return fail(TJX_E_ARG, "tensor base is not 16-byte aligned");
@@ -130,7 +130,7 @@ int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtyp
     return fail(TJX_E_ARG, "TMA box inner extent is not a multiple of 16 bytes");
   CUresult r = fn(out, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox, gelem,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  behind);
   if (r != CUDA_SUCCESS) return fail(TJX_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
   return 0;
 }

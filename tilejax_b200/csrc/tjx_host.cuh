@@ -82,10 +82,11 @@ int* device_status_word();
 long long* profile_buffer(int ctas);
 
 // Encode a tiled tensor map over a row-major bf16/f32 matrix viewed as `rank` dims (innermost first).
-// dims/box in elements, strides in bytes for dims 1..rank-1. Returns 0 or an error code.
+// dims/box in elements, strides in bytes for dims 1..rank-1; `behind` is what a load finds past the matrix (zeros, or NaN).
+// Returns 0 or an error code.
 int make_tensor_map(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int elem_bytes, int rank,
                     const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                    CUtensorMapSwizzle swizzle);
+                    CUtensorMapSwizzle swizzle, CUtensorMapFloatOOBfill behind = CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 
 }  // namespace tjx
 

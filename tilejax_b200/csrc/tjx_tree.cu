@@ -213,6 +213,26 @@ __device__ __forceinline__ uint32_t tree_bits(const TreeMask& mask, int pos, int
   return valid >= 32 ? bits : valid <= 0 ? 0u : bits & ((1u << valid) - 1u);
 }
 
+// Whether a table entry is a page. A position whose entry is not (the planner's -1 where it had none left) is seen by no row. Its
+// copies start behind the cache, which makes its keys NaN and its values zero: its score says so by itself, and nobody has
+// to look the table over beforehand (done by the producers, a vote a block, single tokens took a tenth longer). Whoever
+// meets a score that is NaN looks the block's entries up.
+__device__ __forceinline__ bool tree_is_page(const TreeParams& p, int entry) {
+  return static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_pages);
+}
+
+// Bits of the positions of the block at kv0 that have a page (by a whole warp; pages end at multiples of 16).
+__device__ __forceinline__ uint2 tree_paged(const TreeParams& p, int s, int kv0) {
+  const int lane = threadIdx.x & 31;
+  bool paged = false;
+  if (lane < TR_BLOCK / 16) {
+    const int entry = min((kv0 + 16 * lane) / p.page_size, p.pages_per_seq - 1);
+    paged = tree_is_page(p, p.page_indices[static_cast<size_t>(s) * p.pages_per_seq + entry]);
+  }
+  const uint32_t v = __ballot_sync(0xFFFFFFFFu, paged);
+  return make_uint2((v & 1 ? 0xFFFFu : 0u) | (v & 2 ? 0xFFFF0000u : 0u), (v & 4 ? 0xFFFFu : 0u) | (v & 8 ? 0xFFFF0000u : 0u));
+}
+
 // A whole warp's bounded wait, with one outcome for all lanes; a phase that is there already costs one test and one vote.
 __device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
   if (__builtin_expect(__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity) != 0), 1)) return true;
@@ -232,7 +252,8 @@ __device__ __forceinline__ void tree_zeros(__nv_bfloat162& sum, uint32_t x) {
 }
 
 __global__ void __launch_bounds__(TR_THREADS, 1)
-    tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const TreeParams p) {
+    tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const TreeParams p) {
   using L = TreeSmem;
   extern __shared__ __align__(1024) uint8_t base_ptr[];
   const uint32_t base = smem_u32(base_ptr);
@@ -284,7 +305,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_kv);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_holder)), 512);
@@ -355,6 +377,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
   if (warp == 0 || warp == 11) {
     // ------------------------------------------------------------------ producers: of Q and K, of V
     const bool keys = warp == 0;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
     bool ok = true;
     int qc = 0;      // Q tiles loaded so far
     int block = 0;   // blocks loaded so far
@@ -368,7 +391,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     while (ok && walk.next(p, u)) {
       const int32_t* table = p.page_indices + static_cast<size_t>(u.s) * p.pages_per_seq;
       // The page of this lane's box of block j, and the box's first row there: fetched a block ahead. (An entry past the
-      // table or a page past the pool is clamped, as a gather's index is.)
+      // table is clamped: its positions are past the sequence's end.)
       int page = 0, page_row = 0;
       auto fetch = [&](int j) {
         const int pos = j * TR_BLOCK + lane * p.box_rows;
@@ -393,7 +416,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
       }
       for (int j = u.j0; j < u.j1 && ok; ++j, ++block) {
-        const int row = min(max(page, 0), p.num_pages - 1) * p.page_size + page_row;
+        const int row = tree_is_page(p, page) ? page * p.page_size + page_row : p.num_pages * p.page_size;  // (the latter: behind the cache)
         if (looks && j + 1 < u.j1) fetch(j + 1);
         const int slot = block % (keys ? TR_K_STAGES : TR_V_STAGES), use = block / (keys ? TR_K_STAGES : TR_V_STAGES);
         const uint32_t full = keys ? k_full(slot) : v_full(slot), empty = keys ? k_empty(slot) : v_empty(slot);
@@ -413,8 +436,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < TR_BLOCK / 16; ++i) {
             if (i >= boxes) break;
-            tma_load_3d(dst + i * box_bytes, &map_kv, 0, head, rows[i], full);
-            tma_load_3d(dst + i * box_bytes + L::KV_BYTES / 2, &map_kv, 64, head, rows[i], full);
+            tma_load_3d(dst + i * box_bytes, map, 0, head, rows[i], full);
+            tma_load_3d(dst + i * box_bytes + L::KV_BYTES / 2, map, 64, head, rows[i], full);
           }
         }
         __syncwarp();
@@ -548,24 +571,35 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
           tmem_ld32(s_tmem, v[0]);
           tmem_ld32(s_tmem + 32, v[1]);
           tmem_wait_ld();
-          if (masked.value) {
+          float m_blk;
+          for (bool looked_up = false;; looked_up = true) {
+            if (masked.value) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!((see0 >> i) & 1)) v[0][i] = __float_as_uint(-INFINITY);
-              if (!((see1 >> i) & 1)) v[1][i] = __float_as_uint(-INFINITY);
+              for (int i = 0; i < 32; ++i) {
+                if (!((see0 >> i) & 1)) v[0][i] = __float_as_uint(-INFINITY);
+                if (!((see1 >> i) & 1)) v[1][i] = __float_as_uint(-INFINITY);
+              }
             }
+            // (Maxima of two: 64 of them and the exponentials take two warps of a scheduler 830 cycles, 32 maxima of three 1030.)
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mx[i & 3] = fmax_nan(mx[i & 3], __uint_as_float(v[h][i]));
+            m_blk = fmax_nan(fmax_nan(mx[0], mx[1]), fmax_nan(mx[2], mx[3])) * p.scale_log2e;
+            if (!masked.value || looked_up || __builtin_expect(!__any_sync(0xFFFFFFFFu, mine_valid && m_blk != m_blk), 1)) break;
+            const uint2 paged = tree_paged(p, u.s, (u.j0 + block) * TR_BLOCK);
+            see0 &= paged.x, see1 &= paged.y;
           }
-          // (Maxima of two: 64 of them and the exponentials take two warps of a scheduler 830 cycles, 32 maxima of three 1030.)
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmax_nan(mx[i & 3], __uint_as_float(v[h][i]));
-          float m_blk = fmax_nan(fmax_nan(mx[0], mx[1]), fmax_nan(mx[2], mx[3])) * p.scale_log2e;
           if (m_blk == INFINITY) m_blk = NAN;
           // (Rows of the tile that are none hold other sequences' queries, in place even while those change: they have no say.)
           if (last_job < 0 || __builtin_expect(__any_sync(0xFFFFFFFFu, mine_valid && !(m_blk <= m_used + TR_RESCALE)), 0)) {
             const float m_new = fmax_nan(m_used, m_blk), alpha = ex2(m_used - m_new);
+            if (!masked.value && __any_sync(0xFFFFFFFFu, mine_valid && m_blk != m_blk)) {  // (a NaN raises the maximum)
+              const uint2 paged = tree_paged(p, u.s, (u.j0 + block) * TR_BLOCK);
+              again = (paged.x & paged.y) != 0xFFFFFFFFu;
+              if (again) return;
+            }
             if (!far && __any_sync(0xFFFFFFFFu, mine_valid && tree_far(m_new))) {
               far = true;
               again = !masked.value;
@@ -625,8 +659,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       };
       int block = u.two ? 0 : (t - blocks) & 1;
       const int step = u.two ? 1 : 2;
-      // Blocks that every row sees whole, while no maximum is far from zero (the second loop rounds such scores: 64 products more,
-      // whose code in this one would cost more than they do).
+      // Blocks that every row sees whole, up to one that has positions without a page, and while no maximum is far from zero
+      // (the second loop rounds such scores: 64 products more, whose code in this one would cost more than they do).
       const int plain = min(max(min(u.ctx, u.end) / TR_BLOCK - u.j0, 0), n_blocks);
       for (; block < plain && ok; block += step, ++c) {
         uint32_t pk[32];
@@ -635,7 +669,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
       }
       // Blocks with positions that some row does not see, or that are none. What a row does not see must not reach it: zero
       // times NaN is NaN. So rows of V past the end are zeroed, and rows holding anything but finite numbers too, which are
-      // then added by hand to the rows that see them.
+      // then added by hand to the rows that see them. (None of that where the first loop has left a block: its rows are all seen, or
+      // zero.)
       for (; block < n_blocks && ok; block += step, ++c) {
         const int kv0 = (u.j0 + block) * TR_BLOCK, stage = (blocks + block) % TR_V_STAGES;
         uint32_t bad[4] = {};
@@ -962,7 +997,7 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
   p.part_ml = reinterpret_cast<float2*>(w), w += tree_align256(2ull * ctas * p.part_rows * sizeof(float2));
   p.part_o = reinterpret_cast<float4*>(w);
 
-  CUtensorMap mq, mkv;
+  CUtensorMap mq, mk, mv;
   {
     const uint64_t dims[3] = {TR_D, static_cast<uint64_t>(H), static_cast<uint64_t>(T)};
     const uint64_t strides[2] = {TR_D * 2, static_cast<uint64_t>(H) * TR_D * 2};
@@ -974,7 +1009,10 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
     const uint64_t dims[3] = {TR_D, static_cast<uint64_t>(Hkv) * 2, static_cast<uint64_t>(num_pages) * page_size};
     const uint64_t strides[2] = {TR_D * 2, static_cast<uint64_t>(Hkv) * 2 * TR_D * 2};
     const uint32_t box[3] = {64, 1, static_cast<uint32_t>(p.box_rows)};
-    if (int rc = make_tensor_map(&mkv, kv_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (int rc = make_tensor_map(&mk, kv_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NAN_REQUEST_ZERO_FMA))
+      return rc;
+    if (int rc = make_tensor_map(&mv, kv_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   }
   static bool configured[64] = {};
@@ -985,7 +1023,7 @@ extern "C" int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void*
     configured[dev & 63] = true;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  tree_kernel<<<ctas, TR_THREADS, TreeSmem::TOTAL, s>>>(mq, mkv, p);
+  tree_kernel<<<ctas, TR_THREADS, TreeSmem::TOTAL, s>>>(mq, mk, mv, p);
   TJX_CUDA(cudaGetLastError());
   TJX_CUDA(launch_chained(tree_join_kernel, dim3(ctas, (p.part_rows + 31) / 32), dim3(TJ_WARPS * 32), 0, s, p));
   return 0;

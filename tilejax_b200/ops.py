@@ -677,7 +677,12 @@ def rpa_plan(ctx_lens: torch.Tensor, q_lens: torch.Tensor, page_indices: torch.T
     is empty. `depths` (tokens,) gives drafted tokens their depth in the tree: the token's position is then ctx_lens[s]
     plus its depth, while its slot stays that of its index. All tensors are int32 vectors. `out` is written instead of
     new tensors; it may not overlap the inputs (keep two steps and change over: `rpa_commit` turns kv_lens back into
-    ctx_lens)."""
+    ctx_lens).
+
+    Tokens that get no page (n_free[1] counts the pages that were missing) have slot -1, and are in kv_lens all the same.
+    `rpa_norm_rope_write` writes nothing for them, `rpa_commit` moves nothing, and in `rpa_tree_attention` no row sees
+    them. They are not in the cache: bring them again. `rpa_decode` and `rpa_prefill` clamp such an entry, as a gather
+    does: leave the sequence out of theirs."""
     return RpaStep._make(_native().rpa_plan(ctx_lens, q_lens, page_indices, free_pages, n_free, page_size, tokens,
                                             pages_held, depths, out))
 
@@ -714,8 +719,8 @@ def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.T
     """`rpa_decode` for sequences that bring several drafted tokens each: sequence s < distribution[0] has the tokens
     cu_q_lens[s] .. cu_q_lens[s + 1] - 1 of q (T, H, D), written to the cache behind the others of its kv_lens[s]
     positions. Token t attends to every position before its sequence's new tokens and to those new tokens j whose bit
-    (bit j % 32 of word j // 32) is set in tree_mask[t], int32 (T, words): its ancestors and itself. Their rows become
-    the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
+    (bit j % 32 of word j // 32) is set in tree_mask[t], int32 (T, words): its ancestors and itself; a position whose
+    page_indices entry is no page of the cache (-1) is seen by none. Their rows become the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
     the sequences from distribution[0] on. `out=q` updates in place."""
     return _native().rpa_tree_attention(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution, sm_scale, out)
 
