@@ -312,7 +312,8 @@ int tjx_rpa_plan(const int32_t* ctx_lens, const int32_t* q_lens, const int32_t* 
  * sines; the position is clamped to the table); all in f32, rounded to bf16 once. Pair i is elements i and i + rot / 2,
  * or 2 i and 2 i + 1 if interleaved; elements from rot on are only normed.
  *   q [T, H, D], k, v [T, Hkv, D] bf16, the last dimension dense; strides (HOST) = {q, k, v, q_out, k_out} x {token,
- *   head} in elements, multiples of 4; q_gamma, k_gamma [D] bf16; q_out may be q, k_out may be k
+ *   head} in elements, multiples of 4; q_gamma, k_gamma [D] bf16; q_out may be q, k_out may be k, and
+ *   nothing else that is written may overlap what is read
  *   to a cache: k_out NULL; k and v go to row slots[t] of kv_cache [n_slots, Hkv, 2, D] (a slot out of range writes
  *   nothing; slots are distinct). Without one: v, slots and kv_cache NULL, k goes to k_out.
  * Constraints: D 64, 128 or 256; rot % 8 == 0. */

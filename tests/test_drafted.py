@@ -135,6 +135,35 @@ def test_norm_rope_refusals():
     ])
 
 
+def test_norm_rope_refuses_outputs_among_what_it_looks_up():
+    # Other warps may still read the gammas, positions, angles and slots while one writes.
+    memory = torch.zeros(1 << 14, dtype=torch.bfloat16)
+    ints, floats = memory.view(torch.int32), memory.view(torch.float32)
+
+    def good():
+        return dict(q=heads(3, 4, 128), k=heads(3, 2, 128), q_gamma=heads(128), k_gamma=heads(128), positions=i32(0, 1, 2),
+                    cos_sin=torch.zeros(8, 128))
+
+    def good_write():
+        return dict(**good(), v=heads(3, 2, 128), kv_cache=heads(4, 16, 2, 2, 128), slots=i32(3, 4, 5))
+
+    looked_up = dict(q_gamma=memory[:128], k_gamma=memory[128:256], positions=ints[100:103], cos_sin=floats[4:1028].view(8, 128),
+                     slots=ints[200:203])
+    q_out, k_out = memory[: 3 * 4 * 128].view(3, 4, 128), memory[: 3 * 2 * 128].view(3, 2, 128)
+    for name, tensor in looked_up.items():
+        if name != "slots":
+            for out in ((q_out, heads(3, 2, 128)), (heads(3, 4, 128), k_out)):
+                with pytest.raises(ValueError, match="overlaps"):
+                    ops.qk_norm_rope(**{**good(), name: tensor}, out=out)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.rpa_norm_rope_write(**{**good_write(), name: tensor}, out=q_out)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.rpa_norm_rope_write(**{**good_write(), name: tensor, "kv_cache": memory[: 2 * 16 * 2 * 2 * 128].view(2, 16, 2, 2, 128)})
+    # Side by side is fine: what is left to refuse is the CPU.
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ops.qk_norm_rope(**{**good(), "q_gamma": memory[3 * 4 * 128 : 3 * 4 * 128 + 128]}, out=(q_out, heads(3, 2, 128)))
+
+
 def test_tree_attention_refusals():
     def good():
         return dict(q=heads(3, 4, 128), kv_cache=heads(4, 16, 2, 2, 128), kv_lens=i32(9, 4), page_indices=i32(0, 1, 2, 3),

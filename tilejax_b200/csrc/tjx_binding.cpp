@@ -254,6 +254,11 @@ PyObject* norm_rope(Args a) {
   require(cos_sin.dim() == 2 && cos_sin.scalar_type() == at::kFloat && cos_sin.size(1) <= D && cos_sin.size(1) % 8 == 0 &&
               cos_sin.size(0) > 0 && address(cos_sin) % 16 == 0,
           "cos_sin is float32 (max_positions, rot), rot a multiple of 8 up to the head dimension, 16-byte aligned");
+  // Every warp reads these while others write. (q, k and v, which a row's own warp reads, below.)
+  for (const at::Tensor* written : {a.optional(11, "out"), cache == nullptr ? a.optional(12, "out") : cache})
+    for (const at::Tensor* read : {q_gamma, k_gamma, &positions, &cos_sin, slots})
+      require(written == nullptr || read == nullptr || !overlap(*written, *read),
+              "an output, or the cache, overlaps the gammas, positions, cos_sin or slots");
   int64_t strides[10] = {hq.token, hq.head, hk.token, hk.head, 0, 0, 0, 0, 0, 0};
   Device device;
   device.add(positions), device.add(cos_sin), device.place(q), device.place(k);
