@@ -345,7 +345,8 @@ int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void* kv_cache, 
  * ctx + paths[s, d] holds, for d < n_accepted[s], IN PLACE, and out_lens[s] = ctx + n_accepted[s]. paths int32[S, P]
  * ascends; a path ends in front of an entry that does not, or that is not one of the q_len nodes. n_accepted[s] < 0: the
  * sequence keeps all its tokens, out_lens[s] = kv_lens[s]. Rows of kv_cache [num_pages, page_size, Hkv, 2, D] through
- * page_indices [S * pages_per_seq]; a row without a page is not moved. out_lens must not overlap an input. */
+ * page_indices [S * pages_per_seq]; a row without a page is not moved. Neither kv_cache nor out_lens may
+ * overlap another operand. */
 int tjx_rpa_commit_bf16(void* kv_cache, const int32_t* kv_lens, const int32_t* page_indices, const int32_t* cu_q_lens,
                         const int32_t* paths, const int32_t* n_accepted, int32_t* out_lens, int S, int P, int Hkv, int D,
                         int page_size, int pages_per_seq, int num_pages, tjx_stream_t stream);

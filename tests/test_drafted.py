@@ -195,3 +195,18 @@ def test_commit_refusals():
         ("paths is", "paths", lambda t: t.long()),
         ("n_accepted", "n_accepted", lambda t: t[:1]),
     ])
+
+
+def test_commit_refuses_a_cache_among_its_tables():
+    # Each sequence's block reads its own lengths, path and entries while others move rows.
+    memory = torch.zeros(1 << 15, dtype=torch.bfloat16)
+    ints = memory.view(torch.int32)
+    good = dict(kv_cache=memory[: 2 * 16 * 2 * 2 * 128].view(2, 16, 2, 2, 128), kv_lens=i32(9, 4), page_indices=i32(0, 1, 2, 3),
+                cu_q_lens=i32(0, 2, 3), paths=torch.zeros(2, 2, dtype=torch.int32), n_accepted=i32(1, 1))
+    inside = dict(kv_lens=ints[:2], page_indices=ints[40:44], cu_q_lens=ints[8189:8192], paths=ints[10:14].view(2, 2),
+                  n_accepted=ints[100:102])
+    for name, tensor in inside.items():
+        with pytest.raises(ValueError, match="the cache overlaps"):
+            ops.rpa_commit(**{**good, name: tensor})
+    with pytest.raises(ValueError, match="CUDA tensors"):  # behind it is fine
+        ops.rpa_commit(**{**good, "paths": ints[8192:8196].view(2, 2)})

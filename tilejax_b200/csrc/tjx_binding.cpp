@@ -357,6 +357,8 @@ PyObject* commit(Args a) {
   require(paths.dim() == 2 && paths.size(0) == c.seqs && paths.size(1) > 0 && paths.scalar_type() == at::kInt &&
               is_vector(n_accepted, c.seqs),
           "paths is int32 (S, P), n_accepted int32 (S,)");
+  for (const at::Tensor* t : {&kv_lens, &page_indices, &cu_q_lens, &paths, &n_accepted})
+    require(!overlap(kv_cache, *t), "the cache overlaps kv_lens, page_indices, cu_q_lens, paths or n_accepted");
   Device device;
   for (const at::Tensor* t : {&kv_cache, &kv_lens, &page_indices, &cu_q_lens, &paths, &n_accepted}) device.add(*t);
   at::Tensor out;
