@@ -31,11 +31,11 @@ def pytest_collection_modifyitems(config, items):
 
 @pytest.fixture(scope="session")
 def native():
-    """The built C-ABI library (built on demand where nvcc exists)."""
+    """The built C-ABI library (built on demand where nvcc exists), and its compiled host side as its source is now."""
     from tilejax_b200 import _lib
+    from tilejax_b200.csrc.build import build, build_binding
 
     if not _lib.LIBRARY.exists():
-        from tilejax_b200.csrc.build import build
-
         build()
+    build_binding()
     return _lib.library()

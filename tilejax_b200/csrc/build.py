@@ -77,12 +77,21 @@ def build(force: bool = False, verbose: bool = False, defines: tuple[str, ...] =
 
 
 BINDING = PACKAGE / "_binding.so"
+BINDING_KEY = CSRC / "build" / "binding.key"  # what the file was built for
 
 
-def build_binding(verbose: bool = False) -> Path:
+def binding_key() -> str:
+    """What a build of tjx_binding.cpp depends on beside its sources: it takes torch's classes as its headers lay them out."""
+    import torch
+
+    return f"{sys.implementation.cache_tag} torch-{torch.__version__} cxx11abi-{int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> Path:
     """Compile tjx_binding.cpp (the CPython host side of the drafted-step operators) into _binding.so in the package."""
-    source = CSRC / "tjx_binding.cpp"
-    if _stale(BINDING, [source, (CSRC / "../../include/tilejax_b200.h").resolve(), Path(__file__).resolve()]):
+    source, key = CSRC / "tjx_binding.cpp", binding_key()
+    if (force or _stale(BINDING, [source, (CSRC / "../../include/tilejax_b200.h").resolve(), Path(__file__).resolve()]) or
+            not BINDING_KEY.exists() or BINDING_KEY.read_text() != key):
         import sysconfig
 
         import torch
@@ -92,6 +101,7 @@ def build_binding(verbose: bool = False) -> Path:
                     Path(nvcc()).resolve().parent.parent / "include"]
         fresh = BINDING.with_suffix(".so.new")
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f'-DTJX_BUILT_FOR="{key}"',
                *[f"-I{i}" for i in includes], str(source), "-o", str(fresh), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
                "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"]
         if verbose:
@@ -100,6 +110,8 @@ def build_binding(verbose: bool = False) -> Path:
         if done.returncode != 0:
             raise RuntimeError("g++ failed:\n" + done.stdout)
         os.replace(fresh, BINDING)
+        BINDING_KEY.parent.mkdir(parents=True, exist_ok=True)
+        BINDING_KEY.write_text(key)
     return BINDING
 
 
@@ -143,6 +155,6 @@ if __name__ == "__main__":
     os.chdir(CSRC)
     print(build(args.force, args.verbose, tuple(args.defines), output))
     if output is None:
-        print(build_binding(args.verbose))
+        print(build_binding(args.verbose, args.force))
     if args.ffi:
         print(build_ffi(args.verbose) or "jax.ffi.include_dir() is not available: the handler library was not built")

@@ -418,4 +418,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding(void) { return PyModule_Create(&module); }
+// `built_for`: the Python and torch whose headers this was compiled against (build.py's binding_key).
+PyMODINIT_FUNC PyInit__binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", TJX_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -643,8 +643,13 @@ def _native():
     the C ABI; refusals are ValueError, the library's errors NativeError."""
     global _binding
     if _binding is None:
+        from .csrc.build import binding_key
+
         try:
             from . import _binding as module
+
+            if getattr(module, "built_for", None) != binding_key():
+                raise ImportError(f"built for {getattr(module, 'built_for', 'an unknown torch')}, here is {binding_key()}")
         except ImportError as e:
             raise RuntimeError("tilejax_b200/_binding.so is missing or of another Python or torch: build it with "
                                "`python -m tilejax_b200.csrc.build`") from e
