@@ -708,3 +708,86 @@ def test_two_steps_of_drafted_tokens_with_a_prompt_beside_them():
     want, size = oracle.tree_attention_f64(*host, [3, 3, 3], scale)
     close(to_host(out), want, size, 2.0**-8 + 2.0**-11)
     assert to_host(second.n_free)[1] == 0
+
+
+def test_a_captured_step_of_all_four_follows_its_inputs():
+    # Plan, norm and write, attention and commit in one graph, replayed with other lengths, stacks, tables, masks, paths and data
+    # copied into the same tensors. In the last one the stack runs out: the sequence that lacks pages sees what it has. Each
+    # replay is checked against the oracles, from the cache as it was.
+    S, H, Hkv, page, pps, T, P, scale = 3, 8, 2, 16, 12, 40, 6, 128**-0.5
+    pool = 30
+    table = angles(300, 128)
+    gammas = [rand_bf16((128,), i) for i in (1, 2)]
+
+    def case(seed, ctx, new, n_free):
+        rng = np.random.default_rng(seed)
+        held = [-(-c // page) for c in ctx]
+        order = rng.permutation(pool)
+        pages = np.full((S, pps), -1, np.int32)
+        at = 0
+        for s, n in enumerate(held):
+            pages[s, :n] = order[at : at + n]
+            at += n
+        sees = [tree(n, rng) for n in new]
+        mask, depths = np.zeros((T, 1), np.int32), np.zeros(T, np.int32)
+        mask[: sum(new)] = np.concatenate([oracle.pack_tree_mask(s) for s in sees])
+        depths[: sum(new)] = np.concatenate([s.sum(1) - 1 for s in sees])
+        paths, accepted = np.zeros((S, P), np.int32), np.zeros(S, np.int32)
+        for s, x in enumerate(sees):
+            deepest = np.flatnonzero(x[int(x.sum(1).argmax())])[:P]
+            paths[s, : len(deepest)], accepted[s] = deepest, len(deepest)
+        free = np.zeros(pool, np.int32)
+        free[: pool - at] = order[at:]
+        return dict(ctx=np.array(ctx, np.int32), new=np.array(new, np.int32), pages=pages.reshape(-1), free=free,
+                    n_free=np.array([pool - at if n_free is None else n_free], np.int32), held=np.array(held, np.int32), depths=depths,
+                    mask=mask, paths=paths, accepted=accepted, qkv=rand_bf16((T, H + 2 * Hkv, 128), seed),
+                    cache=rand_bf16((pool, page, Hkv, 2, 128), seed + 50))
+
+    cases = [case(1, [100, 31, 0], [12, 9, 17], None), case(2, [1, 150, 16], [1, 30, 4], None), case(3, [40, 90, 70], [8, 20, 12], 1)]
+    dev = {k: to_device(v) for k, v in cases[0].items()}
+    dist, cos_sin = dev32([S, S, S]), to_device(table)
+    dgammas = [to_device(g) for g in gammas]
+
+    def step():
+        d = dev
+        plan = ops.rpa_plan(d["ctx"], d["new"], d["pages"], d["free"], d["n_free"], page, T, pages_held=d["held"], depths=d["depths"])
+        q, k, v = d["qkv"][:, :H], d["qkv"][:, H : H + Hkv], d["qkv"][:, H + Hkv :]
+        turned, _ = ops.rpa_norm_rope_write(q, k, v, *dgammas, plan.positions, cos_sin, d["cache"], plan.slots)
+        apart = ops.qk_norm_rope(q, k, *dgammas, plan.positions, cos_sin)
+        out = ops.rpa_tree_attention(turned, d["cache"], plan.kv_lens, d["pages"], plan.cu_q_lens, d["mask"], dist, scale)
+        lens = ops.rpa_commit(d["cache"], plan.kv_lens, d["pages"], plan.cu_q_lens, d["paths"], d["accepted"])
+        return plan, turned, apart, out, lens
+
+    def load(c):
+        for k, v in c.items():
+            dev[k].copy_(to_device(v))
+
+    step()
+    load(cases[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, turned, apart, out, lens = step()
+    for c in (*cases, cases[1]):
+        load(c)
+        graph.replay()
+        want = oracle.rpa_plan_ref(c["ctx"], c["new"], c["pages"], c["free"], c["n_free"], page, T, c["held"], c["depths"])
+        for g, w in zip((*plan, dev["pages"]), want):
+            np.testing.assert_array_equal(to_host(g), w)
+        kv_lens, cu, positions, slots, _, left, pages = want
+        assert (left[1] > 0) == (c is cases[2])
+        q, size = oracle.norm_rope_f64(c["qkv"][:, :H], gammas[0], positions, table, 1e-6, False)
+        close(to_host(turned), q, size)
+        assert torch.equal(apart[0], turned)
+        k, size = oracle.norm_rope_f64(c["qkv"][:, H : H + Hkv], gammas[1], positions, table, 1e-6, False)
+        close(to_host(apart[1]), k, size)
+        cache = c["cache"].copy()
+        rows = cache.reshape(-1, Hkv, 2, 128)
+        for t in np.flatnonzero(slots >= 0):
+            rows[slots[t], :, 0], rows[slots[t], :, 1] = to_host(apart[1])[t], c["qkv"][t, H + Hkv :]
+        want_out, size = oracle.tree_attention_f64(to_host(turned), cache, kv_lens, pages, cu, c["mask"], [S] * 3, scale)
+        close(to_host(out), want_out, size, 2.0**-8 + 2.0**-11)
+        want_lens, cache = oracle.rpa_commit_ref(cache, kv_lens, pages, cu, c["paths"], c["accepted"])
+        np.testing.assert_array_equal(to_host(lens), want_lens)
+        np.testing.assert_array_equal(to_host(dev["cache"]).view(np.uint16), cache.view(np.uint16))
+    assert ops.device_status() == 0
