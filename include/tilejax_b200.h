@@ -332,7 +332,8 @@ size_t tjx_rpa_tree_attention_workspace_bytes(int T, int S, int H, int Hkv);
  * words is seen by none, and so is a position whose entry of page_indices is no page of the cache, as tjx_rpa_plan's -1
  * (tjx_rpa_decode_bf16 and tjx_rpa_prefill_bf16 clamp such an entry, as the reference's gather does). A row that sees
  * nothing is zero; what hidden positions hold, NaN included, does not reach the result. Every other row of out [T, H, D] is q's (out may be q), as after tjx_rpa_decode_bf16: tjx_rpa_prefill_bf16
- * with out as its q then serves the sequences from distribution[0] on.
+ * with out as its q then serves the sequences from distribution[0] on, where it takes the cache (pages of 128, H / Hkv
+ * even); elsewhere a prompt's chunk is a path, row i's mask the bits up to i.
  *   workspace: at least tjx_rpa_tree_attention_workspace_bytes(...) bytes, 256-byte aligned
  * Constraints: D == 128; H a multiple of Hkv, H / Hkv <= 128; page_size a multiple of 16; sm_scale > 0. */
 int tjx_rpa_tree_attention_bf16(const void* q, void* out, const void* kv_cache, const int32_t* kv_lens,

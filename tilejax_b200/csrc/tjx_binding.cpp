@@ -1,6 +1,6 @@
 // The host side of the drafted-step operators (tilejax_b200/ops.py: rpa_plan, qk_norm_rope, rpa_norm_rope_write,
 // rpa_tree_attention, rpa_commit) as a CPython module: arguments checked, outputs and scratch allocated, the C ABI called
-// on the tensors' device and its current stream. Their kernels take 4 to 13 us on a small step, and checking the arguments
+// on the tensors' device and its current stream. Their kernels take 3 to 11 us on a small step, and checking the arguments
 // from Python, a query at a time, and passing them through ctypes took 11 to 18.
 //
 // The library's entry points come as addresses (`bind`), from the library that _lib.py has loaded; a negative return

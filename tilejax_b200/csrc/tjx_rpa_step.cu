@@ -200,7 +200,8 @@ struct NormRopeParams {
 // the next chunk's rows, and the next token's angles, on their way while it works on one. Each row is read once and written
 // once; beside the memory the issue of instructions bounds it: 130 for two rows of 128 (issue slots 60 % busy) where
 // unfolded factors, one element an instruction and shuffles between the halves took 200 (77 %). 4096 tokens of 32 + 8 + 8
-// heads 21.5 us (4.8 TB/s), 16384 of 32 + 8 without a cache 62.5 us (5.4 TB/s). (Loads past the L1, or to be dropped first: as
+// heads 21.5 us, 16384 76 us; 16384 of 32 + 8 without a cache 63 us: 5.6 to 5.9 TB/s behind 3 to 5 us that do not depend on
+// the size. (Loads past the L1, or to be dropped first: as
 // fast or a tenth slower.)
 template <int D, bool NEIGHBOURS>
 __global__ void __launch_bounds__(NR_THREADS, NR_BLOCKS) norm_rope_kernel(const NormRopeParams p) {

@@ -5,7 +5,7 @@
 // over the positions p < kv_len - q_len and the nodes j (position kv_len - q_len + j) with bit j of tree_mask[t] set.
 //
 // The rows (node, query head) that share a KV head share its cache, so a position costs 512 bytes of HBM and, at 128
-// rows of tensor work however few are used, 65 k multiply-adds: 11.6 ns of one SM's share of the memory rate against
+// rows of tensor work however few are used, 33 k multiply-adds: 11.6 ns of one SM's share of the memory rate against
 // 5.8 of its tensor rate. So one kernel serves one node and many: whole 128-row tcgen05 tiles, padded.
 //
 // A unit is (sequence, KV head, up to 256 rows): its rows make one tile of 128, or two that share every K / V block of
@@ -24,13 +24,13 @@
 // which they join in TMEM at the end of the unit. TMEM: each group has two score buffers of 64 columns (P, bf16, overlays
 // the scores), so that the next scores are made while it works, and 128 columns of output.
 //
-// What it reaches: one token a sequence over 64 caches of 1000 to 8100 positions 194 us, 6.1 TB/s of the cache, on pages
-// of 16 as on pages of 128; trees of 16 over 32 caches of up to 4096 62 us; trees of 64 (both row tiles full) over two
-// caches of 125 k 265 us, 0.97 PFLOP/s, and 318 us repeated for a second: then the GPU is at its power limit (1000 W, 1.5 GHz).
+// What it reaches: one token a sequence over 64 caches of 1000 to 8100 positions 191 us on pages of 128 and 193 on pages of 16,
+// 6.2 TB/s of the cache; trees of 16 over 32 caches of up to 4096 61 us; trees of 64 (both row tiles full) over two caches of
+// 125 k 266 us, 0.97 PFLOP/s, and 317 us repeated: then the GPU is at its power limit (1000 W, 1.5 GHz).
 // There blocks of 128 positions (whose scores' products read Q from shared memory half as often: 512 cycles for 832, but
 // one score buffer a group) took the same time, repeated and alone, and so did all exponentials on one pipe. What a unit
-// takes beside its blocks is to a large part code that is not in the instruction cache when its turn comes: less of it (104 to
-// 89 KB) made every call shorter, by 3 to 5 %.
+// takes beside its blocks is to a large part code that is not in the instruction cache when its turn comes: a seventh less of
+// it made every call shorter, by 3 to 5 %.
 //
 // A wait tells a barrier's phase from the one before it only. So whoever waits on a ring slot must have seen its use
 // before: rings have an even number of slots and blocks keep their parity over the whole run, so that a group finds
@@ -877,8 +877,8 @@ constexpr int TJ_BATCH = 4;
 
 // The units that several CTAs shared: a CTA per 32 rows (a lane's) joins their partial results in the order of the
 // blocks, a warp 16 of the columns. And the rows that no unit has, which stay the query (CTAs of the first rows only: the
-// others' exit would wait for the lengths). Bound by latency, a unit's entry and then its parts: 2 us of a call of one
-// sequence, 3 to 5 of larger ones (no launch of it at all: 1 us less than one that returns at once).
+// others' exit would wait for the lengths). Bound by latency, a unit's entry and then its parts: 2.5 us of a call of one
+// sequence, 5 of larger ones, of which a launch that returns at once is 0.5 and 0.5 to 1.3.
 __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
   int lo = 0, hi = 0;  // the rows that units have (from arrays that were there before either kernel)
   if (blockIdx.y == 0) {

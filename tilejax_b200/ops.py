@@ -725,8 +725,10 @@ def rpa_tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, kv_lens: torch.T
     cu_q_lens[s] .. cu_q_lens[s + 1] - 1 of q (T, H, D), written to the cache behind the others of its kv_lens[s]
     positions. Token t attends to every position before its sequence's new tokens and to those new tokens j whose bit
     (bit j % 32 of word j // 32) is set in tree_mask[t], int32 (T, words): its ancestors and itself; a position whose
-    page_indices entry is no page of the cache (-1) is seen by none. Their rows become the outputs (zero for a row that sees nothing), every other row stays the query: `rpa_prefill` with out=out serves
-    the sequences from distribution[0] on. `out=q` updates in place."""
+    page_indices entry is no page of the cache (-1) is seen by none. Their rows become the outputs (zero for a row that
+    sees nothing), every other row stays the query: `rpa_prefill` with out=out serves the sequences from distribution[0]
+    on, where it takes the cache (pages of 128, an even number of query heads per KV head); elsewhere a prompt's chunk is
+    a path here, row i's mask the bits up to i. `out=q` updates in place."""
     return _native().rpa_tree_attention(q, kv_cache, kv_lens, page_indices, cu_q_lens, tree_mask, distribution, sm_scale, out)
 
 
